@@ -1,4 +1,4 @@
-"""ctypes wrapper for the gfx950 utility kernels (hip/hiputil.hip).
+"""ctypes wrapper for the gfx950 kernels (hip/hiputil.hip, hip/kvcache.hip).
 
 GPU-only: importing is safe anywhere, calling load() requires a box
 with an MI355X and the built libnvshare_hiputil.so.
@@ -10,6 +10,48 @@ import ctypes
 from dataclasses import dataclass
 
 from nvshare_amd.paths import artifacts
+
+
+def _fields(spec: str) -> list:
+    """[(name, ctypes type)] of "type: name name; type: name" text."""
+    kinds = {"ptr": ctypes.c_void_p, "i64": ctypes.c_int64,
+             "int": ctypes.c_int, "f32": ctypes.c_float}
+    got = []
+    for part in spec.split(";"):
+        kind, names = part.split(":")
+        got += [(n, kinds[kind.strip()]) for n in names.split()]
+    return got
+
+
+class KvCache(ctypes.Structure):
+    """struct nvs_kv of hip/kvcache.h."""
+
+    _fields_ = _fields(
+        "ptr: k_cache v_cache k_scale v_scale table lens starts;"
+        "i64: table_row k_page k_slot k_head v_page v_slot v_head;"
+        "int: type cache_type batch total heads kv_heads dim pages"
+        " page_size per_seq")
+
+
+class KvAppend(ctypes.Structure):
+    """struct nvs_kv_append_args of hip/kvcache.h."""
+
+    _fields_ = _fields(
+        "ptr: q k v q_out rotation;"
+        "i64: q_row q_head k_row k_head v_row v_head q_out_row q_out_head"
+        " rotation_row;"
+        "int: rotary interleaved fill")
+
+
+class KvAttend(ctypes.Structure):
+    """struct nvs_kv_attend_args of hip/kvcache.h."""
+
+    _fields_ = _fields(
+        "ptr: q out lse; i64: q_row q_head out_row out_head;"
+        "f32: scale; int: window max_new fill")
+
+
+KV_BF16, KV_FP16, KV_E4M3 = 0, 1, 2
 
 
 @dataclass
@@ -80,6 +122,20 @@ class HipUtil:
             ctypes.c_float(s), ctypes.c_size_t(n_floats), None),
             "stream_triad")
 
+    def kv_append(self, cache: KvCache, args: KvAppend,
+                  stream: int) -> None:
+        self._ck(self.lib.nvs_kv_append(ctypes.byref(cache),
+                                        ctypes.byref(args),
+                                        ctypes.c_void_p(stream)),
+                 "kv_append")
+
+    def kv_attend(self, cache: KvCache, args: KvAttend,
+                  stream: int) -> None:
+        self._ck(self.lib.nvs_kv_attend(ctypes.byref(cache),
+                                        ctypes.byref(args),
+                                        ctypes.c_void_p(stream)),
+                 "kv_attend")
+
     def sync(self) -> None:
         self._ck(self.lib.nvs_hip_sync(), "hipDeviceSynchronize")
 
@@ -103,6 +159,7 @@ def load() -> HipUtil:
                   "nvs_hip_prefetch_chunked",
                   "nvs_touch_pages", "nvs_read_pages", "nvs_busy",
                   "nvs_stream_triad", "nvs_hip_sync",
-                  "nvs_hip_mem_get_info"):
+                  "nvs_hip_mem_get_info", "nvs_kv_append",
+                  "nvs_kv_attend"):
         getattr(lib, fname).restype = ctypes.c_int
     return HipUtil(lib)
