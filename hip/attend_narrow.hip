@@ -1,0 +1,616 @@
+/*
+ * nvshare-amd: attention of a few rows (single tokens, drafts) over a
+ * paged cache.  See kvattend.h for the division of the work.
+ */
+#include "kvattend.h"
+
+namespace {
+
+/*
+ * A block has W waves and NC columns of 16 rows, all in every wave; wave w
+ * takes each W-th tile of 32 keys.  A wave's tiles lie in LDS of its own,
+ * filled by direct loads, so the waves never wait for each other: the next
+ * tile's keys are requested as soon as this one's are read, its values as
+ * soon as this one's are, and the loads of 4 to 16 waves a CU are under
+ * way together.  What the waves have is added up in LDS at the end.
+ */
+template <typename T, typename C, int D, int NC, int W> struct narrow {
+	static constexpr int TILE = NARROW_TILE;
+	static constexpr int RB = D * sizeof(C);  /* bytes of a row in LDS */
+	static constexpr int LR = RB / 16;	  /* lanes that load a row */
+	static constexpr int RI = 64 / LR;	  /* rows of a load */
+	static constexpr int NI = TILE / RI;	  /* loads of a tile */
+	static constexpr int STAGE = W * 2 * TILE * RB;
+	static constexpr int OUT_ROW = D + 4;	  /* floats, off the banks */
+	static constexpr int MERGE = W * 16 * NC * OUT_ROW * 4;
+	static constexpr int LDS = STAGE > MERGE ? STAGE : MERGE;
+	/* Waves that a SIMD holds: as LDS allows, and with 32 rows as the
+	 * registers do. */
+	static constexpr int WAVES = LDS > 80 * 1024 || W == 2 ? 1 :
+				     LDS * 4 <= 158 * 1024 && NC == 1 ?
+								 4 :
+								 2;
+
+	/* Where a row's 16-byte pieces lie: turned about so that the 16
+	 * rows of a read fall on all banks. */
+	static __device__ __forceinline__ int turn_k(int row)
+	{
+		return RB >= 256 ? row & 15 :
+		       RB == 128 ? (row >> 1) & 7 :
+				   (row >> 2) & 3;
+	}
+
+	static __device__ __forceinline__ int turn_v(int row)
+	{
+		if (sizeof(C) == 2)
+			return RB >= 256 ? (row & 7) << 1 :
+					   ((row >> 1) & 3) << 1;
+		return RB == 256 ? (row & 7) | (row >> 4 & 1) << 3 :
+		       RB == 128 ? (row >> 1 & 3) | (row >> 4 & 1) << 2 :
+				   (row >> 2 & 1) | (row >> 4 & 1) << 1;
+	}
+};
+
+template <typename T, typename C, int D, int NC, int W>
+__global__ __launch_bounds__(64 * W, (narrow<T, C, D, NC, W>::WAVES)) void
+narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
+{
+	typedef narrow<T, C, D, NC, W> N;
+	constexpr int TILE = N::TILE, RB = N::RB, NI = N::NI;
+	__shared__ __attribute__((aligned(16))) char lds[N::LDS];
+	__shared__ float tops[W][16 * NC], sums[W][16 * NC];
+	const int lane = threadIdx.x & 63;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int col = lane & 15, quarter = lane >> 4;
+
+	const int kh = blockIdx.x % c.kv_heads;
+	const int part = blockIdx.x / c.kv_heads % p.narrow_parts;
+	const int b = blockIdx.x / c.kv_heads / p.narrow_parts;
+	const int group = c.heads / c.kv_heads;
+	const sequence s = sequence_of(c, b);
+	const int rows = s.count * group;
+
+	if (p.cover == 1)
+		cover_padding<T>(c, a, blockIdx.x, gridDim.x);
+	if (rows > p.narrow_rows)
+		return;
+	/* A sequence with more rows than the caller said goes undivided. */
+	const int most_parts = rows > p.joined_rows ? 1 : p.narrow_parts;
+
+	char *const k_lds = lds + wave * 2 * TILE * RB;
+	char *const v_lds = k_lds + TILE * RB;
+	const int *const table = c.table + (int64_t)b * c.table_row;
+	const float vs = sizeof(C) == 1 ? c.v_scale[kh] : 1.f;
+	const factor f = factor_of(a.scale * 1.44269504f *
+				   (sizeof(C) == 1 ? c.k_scale[kh] : 1.f));
+	/* Which 16 bytes of a tile's rows this lane loads. */
+	const int lr = lane / N::LR, lc = lane % N::LR;
+
+	for (int r0 = 0; r0 < rows; r0 += 16 * NC) {
+		const int i0 = r0 / group;
+		const int i1 = min(s.count, (r0 + 16 * NC - 1) / group + 1) -
+			       1;
+		const key_range k = keys_of(c, a.window, s, i0, i1, TILE,
+					    NARROW_LEAST, most_parts);
+		const int parts = parts_of(k);
+
+		if (part >= parts)
+			continue;
+		const int first = k.first + part * k.per;
+		const int last = min(k.last, first + k.per);
+
+		u32x4 q[NC][D / 32];
+		/* The lane's row sees keys in (low, lim]. */
+		int lim[NC], low[NC];
+#pragma unroll
+		for (int n = 0; n < NC; n++) {
+			const int r = r0 + 16 * n + col;
+			const int i = r / group;
+
+			lim[n] = low[n] = -1;
+			if (r < rows) {
+				const T *src = (const T *)a.q +
+					       (s.first + i) * a.q_row +
+					       (kh * group + r % group) *
+						       a.q_head;
+				lim[n] = (int)max(min(s.pos + i,
+						      (int64_t)k.hi - 1),
+						  (int64_t)-1);
+				if (a.window > 0)
+					low[n] = (int)max(s.pos + i - a.window,
+							  (int64_t)-1);
+#pragma unroll
+				for (int d = 0; d < D / 32; d++) {
+					q[n][d] = *(const u32x4 *)(src +
+								   32 * d +
+								   8 * quarter);
+					q[n][d] = (q[n][d] ^ f.flip) & f.keep;
+				}
+			} else {
+#pragma unroll
+				for (int d = 0; d < D / 32; d++)
+					q[n][d] = u32x4{};
+			}
+		}
+		/* The limits of all rows: keys up to `all` are seen by each
+		 * unless a window ends before. */
+		const int all = (int)min(max(s.pos + i0, (int64_t)-1),
+					 (int64_t)k.hi - 1);
+		const int any_low =
+			a.window > 0 ? (int)max(s.pos + i1 - a.window + 1,
+						(int64_t)0) :
+				       0;
+		const bool alike = s.pos + i0 == s.pos + i1;
+
+		softmax<T> sm[NC];
+		f32x4 out[NC][D / 16];
+#pragma unroll
+		for (int n = 0; n < NC; n++)
+#pragma unroll
+			for (int d = 0; d < D / 16; d++)
+				out[n][d] = f32x4{};
+
+		/* Request a tile's rows.  `pages` has the page of key lane %
+		 * 32 of the tile; whole: all are in the same.  The addresses
+		 * are made anew each time: kept ones would take more
+		 * registers than the results. */
+		auto request = [&](const void *cache, int64_t page_stride,
+				   int64_t slot_stride, int64_t head, int tile,
+				   int pages, bool whole, bool values,
+				   char *to) {
+			constexpr int SIZE = sizeof(C);
+			const int key = tile * TILE;
+			int r = lr;
+
+			if (whole) {
+				const int page =
+					__builtin_amdgcn_readfirstlane(pages);
+				const char *from =
+					(const char *)cache +
+					(page * page_stride +
+					 slot_of(c, p, key) * slot_stride +
+					 kh * head) * SIZE;
+#pragma unroll
+				for (int i = 0; i < NI; i++) {
+					asm volatile("" : "+v"(r));
+					const int row = i * N::RI + r;
+					const int piece =
+						lc ^ (values ? N::turn_v(row) :
+							       N::turn_k(row));
+
+					copy_to_lds(from +
+							    row * slot_stride *
+								    SIZE +
+							    piece * 16,
+						    to + i * 1024);
+				}
+				return;
+			}
+			const char *base = (const char *)cache +
+					   kh * head * SIZE;
+#pragma unroll
+			for (int i = 0; i < NI; i++) {
+				asm volatile("" : "+v"(r));
+				const int row = i * N::RI + r;
+				const int piece = lc ^ (values ?
+								N::turn_v(row) :
+								N::turn_k(row));
+				const int page = __shfl(pages, row);
+				const char *from =
+					base + (page * page_stride +
+						slot_of(c, p, key + row) *
+							slot_stride) *
+						       SIZE;
+
+				if (page < 0)
+					from = (const char *)no_value;
+				copy_to_lds(from + piece * 16, to + i * 1024);
+			}
+		};
+		auto is_whole = [&](int pages, int tile) {
+			return __all(pages >= 0) &&
+			       (c.page_size % TILE == 0);
+		};
+		auto lookup = [&](int tile) {
+			if (tile >= last)
+				return -1;
+			return page_of(c, p, table,
+				       tile * TILE + (lane & (TILE - 1)), k);
+		};
+
+		int t = first + wave;
+		int pages = lookup(t), next = lookup(t + W);
+		bool whole = is_whole(pages, t);
+
+		if (t < last) {
+			request(c.k_cache, c.k_page, c.k_slot, c.k_head, t,
+				pages, whole, false, k_lds);
+			request(c.v_cache, c.v_page, c.v_slot, c.v_head, t,
+				pages, whole, true, v_lds);
+		}
+		for (; t < last; t += W) {
+			const unsigned valid =
+				(unsigned)__ballot(pages >= 0);
+			const int pages1 = next;
+			const bool whole1 = is_whole(pages1, t + W);
+			const bool more = t + W < last;
+			const int key0 = t * TILE;
+
+			next = lookup(t + 2 * W);
+			/* Keys: S^T = K Q^T. */
+			wait_loads<NI>();
+			f32x4 score[NC][2];
+#pragma unroll
+			for (int h = 0; h < 2; h++) {
+#pragma unroll
+				for (int n = 0; n < NC; n++)
+					score[n][h] = f32x4{};
+#pragma unroll
+				for (int d = 0; d < D / 32; d++) {
+					const int row = 16 * h + col;
+					u32x4 w;
+
+					if constexpr (sizeof(C) == 2) {
+						const int piece =
+							(4 * d + quarter) ^
+							N::turn_k(row);
+
+						w = *(const u32x4
+							      *)(k_lds +
+								 row * RB +
+								 piece * 16);
+					} else {
+						const int piece =
+							(2 * d +
+							 (quarter >> 1)) ^
+							N::turn_k(row);
+
+						w = widen8<T>(
+							*(const u32x2
+								  *)(k_lds +
+								     row * RB +
+								     piece * 16 +
+								     (quarter &
+								      1) *
+									     8));
+					}
+#pragma unroll
+					for (int n = 0; n < NC; n++)
+						score[n][h] = mma16<T>(
+							w, q[n][d],
+							score[n][h]);
+				}
+			}
+			wait_lds();
+			if (more)
+				request(c.k_cache, c.k_page, c.k_slot,
+					c.k_head, t + W, pages1, whole1, false,
+					k_lds);
+
+			/* Weights. */
+			const bool masked = valid != ~0u ||
+					    key0 + TILE - 1 > all ||
+					    key0 < any_low;
+			u32x4 weight[NC];
+#pragma unroll
+			for (int n = 0; n < NC; n++) {
+				float x[8];
+
+#pragma unroll
+				for (int h = 0; h < 2; h++)
+#pragma unroll
+					for (int j = 0; j < 4; j++)
+						x[4 * h + j] = score[n][h][j];
+				if (masked) {
+#pragma unroll
+					for (int e = 0; e < 8; e++) {
+						const int j =
+							16 * (e >> 2) +
+							4 * quarter + (e & 3);
+
+						if (!(valid >> j & 1) ||
+						    key0 + j > lim[n] ||
+						    key0 + j <= low[n])
+							x[e] = -INFINITY;
+					}
+				}
+				float most = x[0];
+#pragma unroll
+				for (int e = 1; e < 8; e++)
+					most = fmaxf(most, x[e]);
+				f32x2 y = odd_even_quarters(most);
+				y = halves(fmaxf(y[0], y[1]));
+				most = fmaxf(y[0], y[1]);
+				if (__any(sm[n].behind(most, f.c))) {
+					const float keep =
+						sm[n].follow(most, f.c);
+#pragma unroll
+					for (int d = 0; d < D / 16; d++)
+						out[n][d] *= keep;
+				}
+				const float unit = sm[n].unit(f.c);
+#pragma unroll
+				for (int e = 0; e < 8; e++) {
+					x[e] = __builtin_amdgcn_exp2f(
+						__builtin_fmaf(x[e], f.c,
+							       -unit));
+					sm[n].sum += x[e];
+				}
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+					weight[n][e] = pack2<T>(x[2 * e],
+								x[2 * e + 1]);
+			}
+
+			/* Values: O^T += V^T P^T. */
+			if (more)
+				wait_loads<NI>();
+			else
+				wait_loads<0>();
+			auto value = [&](int d) {
+				if constexpr (sizeof(C) == 2) {
+					const int row = 4 * quarter +
+							(col >> 2);
+					const int piece =
+						(2 * d + ((col & 3) >> 1)) ^
+						N::turn_v(row);
+					const char *at = v_lds + row * RB +
+							 piece * 16 +
+							 (col & 1) * 8;
+					const u32x2 lo = read_keys4(at);
+					const u32x2 hi =
+						read_keys4(at + 16 * RB);
+
+					return u32x4{ lo[0], lo[1], hi[0],
+						      hi[1] };
+				} else {
+					const int n = col >> 1;
+					const int row =
+						(n < 4 ? 0 : 12) +
+						4 * quarter + n;
+					const int piece = d ^ N::turn_v(row);
+
+					return widen8<T>(read_keys8(
+						v_lds + row * RB +
+						piece * 16 + (col & 1) * 8));
+				}
+			};
+			/* The 4 values of key j that go into out[.][d]. */
+			auto four = [&](int j, int d, float *x) {
+				const int byte = (16 * d + 4 * quarter) *
+						 (int)sizeof(C);
+				const char *at =
+					v_lds + j * RB +
+					((byte >> 4) ^ N::turn_v(j)) * 16 +
+					(byte & 15);
+
+				if constexpr (sizeof(C) == 2) {
+					const u32x2 w = *(const u32x2 *)at;
+					const T *v = (const T *)&w;
+#pragma unroll
+					for (int e = 0; e < 4; e++)
+						x[e] = (float)v[e];
+				} else {
+					const unsigned w =
+						*(const unsigned *)at;
+					const f32x2 lo =
+						__builtin_amdgcn_cvt_pk_f32_fp8(
+							w, false);
+					const f32x2 hi =
+						__builtin_amdgcn_cvt_pk_f32_fp8(
+							w, true);
+
+					x[0] = lo[0];
+					x[1] = lo[1];
+					x[2] = hi[0];
+					x[3] = hi[1];
+				}
+			};
+			/* 0 * inf is no number.  Where some rows see a key and
+			 * others do not, and its values are not all finite,
+			 * the rows that see it get these added one by one,
+			 * and the product takes zeros in their place. */
+			bool odd = false;
+
+			if (masked && !alike)
+				for (int i = 0; i < NI; i++) {
+					const u32x4 w =
+						*(const u32x4 *)(v_lds +
+								 i * 1024 +
+								 lane * 16);
+
+					odd |= not_finite<C>(w[0]) |
+					       not_finite<C>(w[1]) |
+					       not_finite<C>(w[2]) |
+					       not_finite<C>(w[3]);
+				}
+			if (__any(odd)) {
+#pragma unroll 1
+				for (int j = 0; j < TILE; j++) {
+					const int key = key0 + j;
+					bool sees[NC];
+
+#pragma unroll
+					for (int n = 0; n < NC; n++)
+						sees[n] = (valid >> j & 1) &&
+							  key <= lim[n] &&
+							  key > low[n];
+#pragma unroll
+					for (int d = 0; d < D / 16; d++) {
+						float x[4];
+
+						asm volatile("" ::: "memory");
+						four(j, d, x);
+#pragma unroll
+						for (int n = 0; n < NC; n++)
+#pragma unroll
+							for (int e = 0; e < 4;
+							     e++)
+								out[n][d][e] +=
+									sees[n] ?
+										odd_only(
+											x[e]) :
+										0.f;
+					}
+				}
+#pragma unroll 1
+				for (int i = 0; i < NI; i++) {
+					u32x4 *at = (u32x4 *)(v_lds + i * 1024 +
+							      lane * 16);
+					u32x4 w = *at;
+
+#pragma unroll
+					for (int e = 0; e < 4; e++)
+						w[e] = finite_only<C>(w[e]);
+					*at = w;
+				}
+				asm volatile("" ::: "memory");
+			}
+#pragma unroll
+			for (int d = 0; d < D / 16; d++) {
+				const u32x4 w = value(d);
+#pragma unroll
+				for (int n = 0; n < NC; n++)
+					out[n][d] = mma16<T>(w, weight[n],
+							     out[n][d]);
+			}
+			wait_lds();
+			if (more)
+				request(c.v_cache, c.v_page, c.v_slot,
+					c.v_head, t + W, pages1, whole1, true,
+					v_lds);
+			pages = pages1;
+			whole = whole1;
+		}
+
+		/* Join the waves. */
+		float *const merge = (float *)lds;
+		const float lift = types<T>::lift;
+
+		__syncthreads(); /* all have read their tiles */
+#pragma unroll
+		for (int n = 0; n < NC; n++) {
+			f32x2 y = odd_even_quarters(sm[n].sum);
+			y = halves(y[0] + y[1]);
+			if (quarter == 0) {
+				tops[wave][16 * n + col] = sm[n].top;
+				sums[wave][16 * n + col] = y[0] + y[1];
+			}
+#pragma unroll
+			for (int d = 0; d < D / 16; d++)
+				*(f32x4 *)(merge +
+					   (wave * 16 * NC + 16 * n + col) *
+						   N::OUT_ROW +
+					   16 * d + 4 * quarter) = out[n][d];
+		}
+		__syncthreads();
+		for (int at = threadIdx.x; at < 16 * NC * (D / 8);
+		     at += 64 * W) {
+			const int r = at / (D / 8), d = at % (D / 8) * 8;
+			const int i = (r0 + r) / group;
+			const int head = kh * group + (r0 + r) % group;
+			float top = -INFINITY, sum = 0.f, x[8] = {};
+
+			if (r0 + r >= rows)
+				continue;
+#pragma unroll
+			for (int w = 0; w < W; w++)
+				top = fmaxf(top, tops[w][r]);
+#pragma unroll
+			for (int w = 0; w < W; w++) {
+				const float *src =
+					merge +
+					(w * 16 * NC + r) * N::OUT_ROW + d;
+				const float m =
+					tops[w][r] == -INFINITY ?
+						0.f :
+						__builtin_amdgcn_exp2f(
+							(tops[w][r] - top) *
+							f.c);
+
+				sum += m * sums[w][r];
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+					x[e] += m * src[e];
+			}
+			const int64_t row = s.first + i;
+			const float unit = top == -INFINITY ? -INFINITY :
+							      top * f.c - lift;
+
+			if (parts > 1) {
+				const int64_t at_row =
+					((part * (int64_t)c.batch + b) *
+						 c.kv_heads +
+					 kh) * p.span +
+					r;
+				f32x4 *o = (f32x4 *)(p.narrow_out +
+						     at_row * D + d);
+
+				o[0] = f32x4{ x[0], x[1], x[2], x[3] };
+				o[1] = f32x4{ x[4], x[5], x[6], x[7] };
+				if (d == 0)
+					p.narrow_sum[at_row] = f32x2{ unit, sum };
+				continue;
+			}
+			const float inv = sum == 0.f ? 0.f : vs / sum;
+			u32x4 o;
+
+#pragma unroll
+			for (int e = 0; e < 4; e++)
+				o[e] = pack2<T>(x[2 * e] * inv,
+						x[2 * e + 1] * inv);
+			*(u32x4 *)((T *)a.out + row * a.out_row +
+				   head * a.out_head + d) = o;
+			if (a.lse && d == 0)
+				a.lse[row * c.heads + head] =
+					sum == 0.f ?
+						-INFINITY :
+						(unit +
+						 __builtin_amdgcn_logf(sum)) *
+							0.693147181f;
+		}
+		__syncthreads(); /* before the next rows' tiles */
+	}
+}
+
+template <typename T, typename C, int D>
+void launch(const nvs_kv &c, const nvs_kv_attend_args &a, const nvs_plan &p,
+	    hipStream_t s)
+{
+	/* Wide rows of 16 bits: half the waves, as their tiles are twice as
+	 * large. */
+	constexpr int W = D * sizeof(C) > 256 ? 2 : 4;
+	const dim3 grid(c.batch * c.kv_heads * p.narrow_parts);
+
+	if (p.span == 16)
+		hipLaunchKernelGGL((narrow_kernel<T, C, D, 1, W>), grid,
+				   dim3(64 * W), 0, s, c, a, p);
+	else
+		hipLaunchKernelGGL((narrow_kernel<T, C, D, 2, W>), grid,
+				   dim3(64 * W), 0, s, c, a, p);
+}
+
+} /* namespace */
+
+template <typename T, typename C>
+hipError_t nvs_narrow(const nvs_kv &c, const nvs_kv_attend_args &a,
+		      const nvs_plan &p, hipStream_t s)
+{
+	if (c.dim == 64)
+		launch<T, C, 64>(c, a, p, s);
+	else if (c.dim == 128)
+		launch<T, C, 128>(c, a, p, s);
+	else
+		launch<T, C, 256>(c, a, p, s);
+	return hipGetLastError();
+}
+
+#define INSTANCE(T, C)                                                     \
+	template hipError_t nvs_narrow<T, C>(const nvs_kv &,               \
+					     const nvs_kv_attend_args &,   \
+					     const nvs_plan &,             \
+					     hipStream_t);
+INSTANCE(bf16_t, bf16_t)
+INSTANCE(bf16_t, e4m3_t)
+INSTANCE(fp16_t, fp16_t)
+INSTANCE(fp16_t, e4m3_t)

@@ -1,0 +1,667 @@
+/*
+ * nvshare-amd: attention of chunks of new tokens over a paged cache, and
+ * the join of divided rows.  See kvattend.h for the division of the work.
+ */
+#include "kvattend.h"
+
+namespace {
+
+/*
+ * Four waves of 32 rows share tiles of 64 keys and values in LDS, two of
+ * each: while one is worked on, the next is on its way.  A 16-bit cache is
+ * loaded there directly; e4m3 goes through registers and lies in LDS as
+ * T, so that each value is widened once and not by each wave.
+ */
+template <typename T, typename C, int D> struct wide {
+	static constexpr int TILE = WIDE_TILE;
+	static constexpr int RB = D * 2;	 /* bytes of a row in LDS */
+	static constexpr int LR = RB / 16;	 /* lanes that load a row */
+	static constexpr int RI = 64 / LR;	 /* rows of a load */
+	static constexpr int NI = TILE / RI / 4; /* a wave's loads of a tile */
+	static constexpr int BUFFER = TILE * RB;
+	static constexpr int LDS = 4 * BUFFER;
+	/* Waves of a SIMD: two blocks a CU, as far as LDS goes. */
+	static constexpr int WAVES = LDS > 80 * 1024 ? 1 : 2;
+	/* e4m3: 16-byte pieces of a thread. */
+	static constexpr int NP = TILE * D / 16 / 256;
+
+	/* Where a row's 16-byte pieces lie, so that reads of 16 rows (keys)
+	 * and of 4 rows' 64 bytes (values) fall on all banks. */
+	static __device__ __forceinline__ int turn_k(int row)
+	{
+		return RB >= 256 ? row & 15 : (row >> 1) & 7;
+	}
+
+	static __device__ __forceinline__ int turn_v(int row)
+	{
+		return RB >= 256 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
+	}
+};
+
+template <typename T, typename C, int D>
+__global__ __launch_bounds__(256, (wide<T, C, D>::WAVES)) void
+wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
+{
+	typedef wide<T, C, D> W;
+	constexpr int TILE = W::TILE, RB = W::RB, NI = W::NI;
+	__shared__ __attribute__((aligned(16))) char lds[W::LDS];
+	__shared__ int odd_tile[2];
+	const int lane = threadIdx.x & 63;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int col = lane & 31, half = lane >> 5;
+
+	/* This block's sequence and rows: sequence b has the blocks from
+	 * starts[b] * group / WIDE_ROWS + b on, which is room enough for
+	 * its own.  The last blocks of rows, which see the most keys, go
+	 * first. */
+	const int group = c.heads / c.kv_heads;
+	const int kh = blockIdx.x % c.kv_heads;
+	const int part = blockIdx.x / c.kv_heads % p.wide_parts;
+	const int at = p.wide_blocks - 1 -
+		       blockIdx.x / c.kv_heads / p.wide_parts;
+	int64_t block;
+	int b;
+
+	if (p.cover == 2)
+		cover_padding<T>(c, a, blockIdx.x, gridDim.x);
+	if (c.starts) {
+		auto from = [&](int i) {
+			return (int64_t)c.starts[i] * group / WIDE_ROWS + i;
+		};
+		if (from(0) > at)
+			return;
+		b = last_at_most(c.batch, at, from);
+		if (b == c.batch)
+			return;
+		block = at - from(b);
+	} else {
+		b = at % c.batch;
+		block = at / c.batch;
+	}
+	const sequence s = sequence_of(c, b);
+	const int rows = s.count * group;
+
+	if (block * WIDE_ROWS >= rows || rows <= p.narrow_rows)
+		return;
+	const int r0 = (int)block * WIDE_ROWS;
+	const int i0 = r0 / group;
+	const int i1 = min(s.count, (r0 + WIDE_ROWS - 1) / group + 1) - 1;
+	const key_range k =
+		keys_of(c, a.window, s, i0, i1, TILE, WIDE_LEAST, p.wide_parts);
+	const int parts = parts_of(k);
+
+	if (part >= parts)
+		return;
+	const int first = k.first + part * k.per;
+	const int last = min(k.last, first + k.per);
+
+	const int *const table = c.table + (int64_t)b * c.table_row;
+	const float vs = sizeof(C) == 1 ? c.v_scale[kh] : 1.f;
+	const factor f = factor_of(a.scale * 1.44269504f *
+				   (sizeof(C) == 1 ? c.k_scale[kh] : 1.f));
+
+	/* The lane's row, and the limits of the wave's. */
+	const int r = r0 + wave * 32 + col;
+	const bool real = r < rows;
+	const int token = r / group, head = kh * group + r % group;
+	auto limit = [&](int i) {
+		return (int)max(min(s.pos + i, (int64_t)k.hi - 1),
+				(int64_t)-1);
+	};
+	/* The row sees keys in (low, lim]. */
+	const int lim = real ? limit(token) : -1;
+	const int low = a.window > 0 ? (int)max(s.pos + token - a.window,
+						(int64_t)-1) :
+				       -1;
+	const int w0 = min(rows - 1, r0 + wave * 32) / group;
+	const int w1 = min(rows - 1, r0 + wave * 32 + 31) / group;
+	const bool idle = r0 + wave * 32 >= rows;
+	const int all = limit(w0), most_lim = limit(w1);
+	const int any_low = a.window > 0 ?
+				    (int)max(s.pos + w1 - a.window + 1,
+					     (int64_t)0) :
+				    0;
+	const int least_low = a.window > 0 ?
+				      (int)max(s.pos + w0 - a.window + 1,
+					       (int64_t)0) :
+				      0;
+	/* Where the block's rows do not all see the same. */
+	const int block_all = limit(i0);
+	const int block_low = a.window > 0 ?
+				      (int)max(s.pos + i1 - a.window + 1,
+					       (int64_t)0) :
+				      0;
+	const bool alike = i0 == i1;
+
+	u32x4 q[D / 16];
+	const T *src = (const T *)a.q + (s.first + token) * a.q_row +
+		       head * a.q_head;
+#pragma unroll
+	for (int d = 0; d < D / 16; d++) {
+		q[d] = u32x4{};
+		if (real)
+			q[d] = *(const u32x4 *)(src + 16 * d + 8 * half);
+		q[d] = (q[d] ^ f.flip) & f.keep;
+	}
+
+	softmax<T> sm;
+	f32x16 out[D / 32];
+#pragma unroll
+	for (int d = 0; d < D / 32; d++)
+#pragma unroll
+		for (int e = 0; e < 16; e++)
+			out[d][e] = 0.f;
+
+	/* The pages of a tile's keys, key lane of it in lane `lane`. */
+	auto lookup = [&](int tile) {
+		if (tile >= last)
+			return -1;
+		return page_of(c, p, table, tile * TILE + lane, k);
+	};
+	auto is_whole = [&](int pages) {
+		return __all(pages >= 0) && c.page_size % TILE == 0;
+	};
+	constexpr int SIZE = sizeof(C);
+	/* Where a tile's row begins in the cache. */
+	auto row_of = [&](const void *cache, int64_t page_stride,
+			  int64_t slot_stride, int64_t head_stride, int key,
+			  int pages, bool whole, int row) {
+		const char *base = (const char *)cache + kh * head_stride * SIZE;
+
+		if (whole) {
+			const int page = __builtin_amdgcn_readfirstlane(pages);
+
+			return base +
+			       (page * page_stride +
+				slot_of(c, p, key) * slot_stride) *
+				       SIZE +
+			       row * slot_stride * SIZE;
+		}
+		const int page = __shfl(pages, row);
+
+		if (page < 0)
+			return (const char *)no_value;
+		return base + (page * page_stride +
+			       slot_of(c, p, key + row) * slot_stride) *
+				      SIZE;
+	};
+	/* 16 bits: request a tile for buffer n. */
+	auto request = [&](int tile, int pages, int n) {
+		const bool whole = is_whole(pages);
+		const int key = tile * TILE;
+		char *to = lds + n * 2 * W::BUFFER + wave * NI * 1024;
+		const int lr = lane / W::LR, lc = lane % W::LR;
+#pragma unroll
+		for (int i = 0; i < NI; i++) {
+			const int row = (wave * NI + i) * W::RI + lr;
+
+			copy_to_lds(row_of(c.k_cache, c.k_page, c.k_slot,
+					   c.k_head, key, pages, whole, row) +
+					    (lc ^ W::turn_k(row)) * 16,
+				    to + i * 1024);
+			copy_to_lds(row_of(c.v_cache, c.v_page, c.v_slot,
+					   c.v_head, key, pages, whole, row) +
+					    (lc ^ W::turn_v(row)) * 16,
+				    to + W::BUFFER + i * 1024);
+		}
+	};
+	/* e4m3: fetch a tile into registers, put it into buffer n. */
+	u32x4 hold[2][SIZE == 1 ? W::NP : 1];
+	auto fetch = [&](int tile, int pages) {
+		const bool whole = is_whole(pages);
+		const int key = tile * TILE;
+#pragma unroll
+		for (int i = 0; i < W::NP; i++) {
+			const int n = i * 256 + threadIdx.x;
+			const int row = n / (D / 16), piece = n % (D / 16);
+
+			hold[0][i] = *(const u32x4 *)(row_of(c.k_cache,
+							     c.k_page, c.k_slot,
+							     c.k_head, key,
+							     pages, whole,
+							     row) +
+						      piece * 16);
+			hold[1][i] = *(const u32x4 *)(row_of(c.v_cache,
+							     c.v_page, c.v_slot,
+							     c.v_head, key,
+							     pages, whole,
+							     row) +
+						      piece * 16);
+		}
+	};
+	auto put = [&](int n) {
+		char *to = lds + n * 2 * W::BUFFER;
+#pragma unroll
+		for (int i = 0; i < W::NP; i++) {
+			const int m = i * 256 + threadIdx.x;
+			const int row = m / (D / 16), piece = m % (D / 16) * 2;
+#pragma unroll
+			for (int e = 0; e < 2; e++) {
+				const u32x4 w = hold[0][i], x = hold[1][i];
+
+				*(u32x4 *)(to + row * RB +
+					   ((piece + e) ^ W::turn_k(row)) *
+						   16) =
+					widen8<T>(u32x2{ w[2 * e],
+							 w[2 * e + 1] });
+				*(u32x4 *)(to + W::BUFFER + row * RB +
+					   ((piece + e) ^ W::turn_v(row)) *
+						   16) =
+					widen8<T>(u32x2{ x[2 * e],
+							 x[2 * e + 1] });
+			}
+		}
+	};
+
+	int pages = lookup(first), next = lookup(first + 1);
+
+	if (first < last) {
+		if constexpr (SIZE == 2) {
+			request(first, pages, 0);
+		} else {
+			fetch(first, pages);
+			put(0);
+		}
+	}
+	for (int t = first; t < last; t++) {
+		const int n = (t - first) & 1;
+		const char *const k_lds = lds + n * 2 * W::BUFFER;
+		char *const v_lds = lds + n * 2 * W::BUFFER + W::BUFFER;
+		const uint64_t valid = __ballot(pages >= 0);
+		const int key0 = t * TILE;
+
+		/* This tile has come, and all are done with the other. */
+		if constexpr (SIZE == 2)
+			wait_loads<0>();
+		wait_lds();
+		__builtin_amdgcn_s_barrier();
+		asm volatile("" ::: "memory");
+		if (t + 1 < last) {
+			if constexpr (SIZE == 2)
+				request(t + 1, next, n ^ 1);
+			else
+				fetch(t + 1, next);
+		}
+		pages = next;
+		next = lookup(t + 2);
+
+		/* 0 * inf is no number: values that are not finite and not
+		 * seen by all rows are added for those that see them, and
+		 * the product takes zeros in their place. */
+		const bool uneven = !alike && (key0 + TILE - 1 > block_all ||
+					       key0 < block_low);
+		if (uneven) {
+			bool odd = false;
+
+			if (threadIdx.x == 0)
+				odd_tile[n] = 0;
+			__syncthreads();
+			for (int i = 0; i < NI; i++) {
+				const u32x4 w = *(
+					const u32x4 *)(v_lds +
+						       (wave * NI + i) * 1024 +
+						       lane * 16);
+
+				odd |= not_finite<T>(w[0]) |
+				       not_finite<T>(w[1]) |
+				       not_finite<T>(w[2]) | not_finite<T>(w[3]);
+			}
+			if (odd)
+				odd_tile[n] = 1;
+			__syncthreads();
+			if (odd_tile[n]) {
+#pragma unroll 1
+				for (int j = 0; j < TILE; j++) {
+					const int key = key0 + j;
+					const bool sees =
+						(valid >> j & 1) &&
+						key <= lim && key > low;
+#pragma unroll
+					for (int d = 0; d < D / 8; d++) {
+						const char *from =
+							v_lds + j * RB +
+							(d ^ W::turn_v(j)) *
+								16 +
+							half * 8;
+						asm volatile("" ::: "memory");
+						const u32x2 w =
+							*(const u32x2 *)from;
+						const T *v = (const T *)&w;
+#pragma unroll
+						for (int e = 0; e < 4; e++)
+							out[d / 4][d % 4 * 4 +
+								   e] +=
+								sees ? odd_only((
+									       float)v[e]) :
+								       0.f;
+					}
+				}
+				__syncthreads();
+#pragma unroll 1
+				for (int i = 0; i < NI; i++) {
+					u32x4 *to = (u32x4 *)(v_lds +
+							      (wave * NI + i) *
+								      1024 +
+							      lane * 16);
+					u32x4 w = *to;
+
+#pragma unroll
+					for (int e = 0; e < 4; e++)
+						w[e] = finite_only<T>(w[e]);
+					*to = w;
+				}
+				__syncthreads();
+			}
+		}
+
+		if (!idle && key0 <= most_lim && key0 + TILE > least_low) {
+			/* Keys: S^T = K Q^T. */
+			f32x16 score[2];
+#pragma unroll
+			for (int h = 0; h < 2; h++) {
+#pragma unroll
+				for (int e = 0; e < 16; e++)
+					score[h][e] = 0.f;
+#pragma unroll
+				for (int d = 0; d < D / 16; d++) {
+					const int row = 32 * h + col;
+					const u32x4 w = *(
+						const u32x4 *)(k_lds +
+							       row * RB +
+							       ((2 * d + half) ^
+								W::turn_k(
+									row)) *
+								       16);
+
+					score[h] = mma32<T>(w, q[d], score[h]);
+				}
+			}
+
+			/* Weights. */
+			if (valid != ~0ull || key0 + TILE - 1 > all ||
+			    key0 < any_low) {
+#pragma unroll
+				for (int h = 0; h < 2; h++)
+#pragma unroll
+					for (int e = 0; e < 16; e++) {
+						const int j =
+							32 * h +
+							8 * (e >> 2) +
+							4 * half + (e & 3);
+
+						if (!(valid >> j & 1) ||
+						    key0 + j > lim ||
+						    key0 + j <= low)
+							score[h][e] =
+								-INFINITY;
+					}
+			}
+			float most = score[0][0];
+#pragma unroll
+			for (int e = 1; e < 16; e++)
+				most = fmaxf(most, score[0][e]);
+#pragma unroll
+			for (int e = 0; e < 16; e++)
+				most = fmaxf(most, score[1][e]);
+			const f32x2 y = halves(most);
+
+			most = fmaxf(y[0], y[1]);
+			if (__any(sm.behind(most, f.c))) {
+				const float keep = sm.follow(most, f.c);
+#pragma unroll
+				for (int d = 0; d < D / 32; d++)
+					out[d] *= keep;
+			}
+			const float unit = sm.unit(f.c);
+			u32x4 weight[4];
+#pragma unroll
+			for (int h = 0; h < 2; h++) {
+#pragma unroll
+				for (int e = 0; e < 16; e++) {
+					score[h][e] = __builtin_amdgcn_exp2f(
+						__builtin_fmaf(score[h][e],
+							       f.c, -unit));
+					sm.sum += score[h][e];
+				}
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+					weight[2 * h + e / 4][e % 4] =
+						pack2<T>(score[h][2 * e],
+							 score[h][2 * e + 1]);
+			}
+
+			/* Values: O^T += V^T P^T. */
+#pragma unroll
+			for (int h = 0; h < 4; h++) {
+				const int row = 16 * h + 4 * half +
+						((lane & 15) >> 2);
+#pragma unroll
+				for (int d = 0; d < D / 32; d++) {
+					const int piece =
+						(4 * d + 2 * (lane >> 4 & 1) +
+						 ((lane & 3) >> 1)) ^
+						W::turn_v(row);
+					const char *from = v_lds + row * RB +
+							   piece * 16 +
+							   (lane & 1) * 8;
+					const u32x2 lo = read_keys4(from);
+					const u32x2 hi =
+						read_keys4(from + 8 * RB);
+
+					out[d] = mma32<T>(u32x4{ lo[0], lo[1],
+								 hi[0],
+								 hi[1] },
+							  weight[h], out[d]);
+				}
+			}
+		}
+		if constexpr (SIZE == 1)
+			if (t + 1 < last)
+				put(n ^ 1);
+	}
+
+	/* The result: lane `col` of each half has 4 of each 8 dimensions. */
+	const f32x2 y = halves(sm.sum);
+	const float sum = y[0] + y[1];
+	const int64_t row = s.first + token;
+	const float unit = sm.top == -INFINITY ? -INFINITY : sm.unit(f.c);
+
+	if (!real)
+		return;
+	if (parts > 1) {
+		const int64_t at_row =
+			(part * (int64_t)c.total + row) * c.heads + head;
+#pragma unroll
+		for (int d = 0; d < D / 8; d++) {
+			const f32x16 x = out[d / 4];
+			const int e = d % 4 * 4;
+
+			*(f32x4 *)(p.wide_out + at_row * D + 8 * d +
+				   4 * half) =
+				f32x4{ x[e], x[e + 1], x[e + 2], x[e + 3] };
+		}
+		if (half == 0)
+			p.wide_sum[at_row] = f32x2{ unit, sum };
+		return;
+	}
+	const float inv = sum == 0.f ? 0.f : vs / sum;
+#pragma unroll
+	for (int d = 0; d < D / 8; d++) {
+		const f32x16 x = out[d / 4];
+		const int e = d % 4 * 4;
+		const u32x2 w = { pack2<T>(x[e] * inv, x[e + 1] * inv),
+				  pack2<T>(x[e + 2] * inv, x[e + 3] * inv) };
+
+		*(u32x2 *)((T *)a.out + row * a.out_row + head * a.out_head +
+			   8 * d + 4 * half) = w;
+	}
+	if (a.lse && half == 0)
+		a.lse[row * c.heads + head] =
+			sum == 0.f ? -INFINITY :
+				     (unit + __builtin_amdgcn_logf(sum)) *
+					     0.693147181f;
+}
+
+/*
+ * Join the parts of rows whose keys were divided: a block to a row, its
+ * threads over the dimensions and then over the parts.  Rows with one part
+ * have their result already.
+ */
+template <typename T, int D, bool NARROW>
+__global__ __launch_bounds__(256) void join_kernel(nvs_kv c,
+						   nvs_kv_attend_args a,
+						   nvs_plan p)
+{
+	constexpr int TD = D / 4, TP = 256 / TD; /* threads: dims, parts */
+	__shared__ f32x4 add[TP][TD];
+	__shared__ float adds[TP];
+	const int td = threadIdx.x % TD, tp = threadIdx.x / TD;
+	const int group = c.heads / c.kv_heads;
+	int b, r, head;
+
+	if (NARROW) {
+		const int item = blockIdx.x / p.joined_rows;
+
+		b = item / c.kv_heads;
+		r = blockIdx.x % p.joined_rows;
+		head = item % c.kv_heads * group + r % group;
+	} else {
+		head = blockIdx.x % c.heads;
+		b = sequence_at(c, blockIdx.x / c.heads);
+		if (b < 0)
+			return;
+	}
+	const sequence s = sequence_of(c, b);
+	const int rows = s.count * group, kh = head / group;
+	int64_t at, step; /* of the row in a part, and between parts */
+
+	if (NARROW) {
+		if (r >= rows || rows > p.joined_rows)
+			return;
+		at = ((int64_t)b * c.kv_heads + kh) * p.span + r;
+		step = (int64_t)c.batch * c.kv_heads * p.span;
+	} else {
+		r = ((int)(blockIdx.x / c.heads) - s.first) * group +
+		    head % group;
+		if (r >= rows || rows <= p.narrow_rows)
+			return;
+		at = blockIdx.x;
+		step = (int64_t)c.total * c.heads;
+	}
+	const int span = NARROW ? p.span : WIDE_ROWS;
+	const int r0 = r / span * span;
+	const key_range k = keys_of(
+		c, a.window, s, r0 / group,
+		min(s.count, (r0 + span - 1) / group + 1) - 1,
+		NARROW ? NARROW_TILE : WIDE_TILE,
+		NARROW ? NARROW_LEAST : WIDE_LEAST,
+		NARROW ? p.narrow_parts : p.wide_parts);
+	const int parts = parts_of(k);
+
+	if (parts < 2)
+		return;
+	const f32x2 *sums = (NARROW ? p.narrow_sum : p.wide_sum) + at;
+	const float *outs = (NARROW ? p.narrow_out : p.wide_out) + at * D +
+			    4 * td;
+	float unit = -INFINITY, sum = 0.f;
+	f32x4 x = {};
+
+	for (int n = 0; n < parts; n++)
+		unit = fmaxf(unit, sums[n * step][0]);
+	for (int n = tp; n < parts; n += TP) {
+		const f32x2 y = sums[n * step];
+		const float m = y[0] == -INFINITY ?
+					0.f :
+					__builtin_amdgcn_exp2f(y[0] - unit);
+
+		sum += m * y[1];
+		x += m * *(const f32x4 *)(outs + n * step * D);
+	}
+	add[tp][td] = x;
+	if (td == 0)
+		adds[tp] = sum;
+	__syncthreads();
+	if (tp)
+		return;
+	sum = adds[0];
+	for (int n = 1; n < TP; n++) {
+		x += add[n][td];
+		sum += adds[n];
+	}
+	const float inv =
+		sum == 0.f ? 0.f : (c.v_scale ? c.v_scale[kh] : 1.f) / sum;
+	const int64_t row = s.first + r / group;
+
+	*(u32x2 *)((T *)a.out + row * a.out_row + head * a.out_head + 4 * td) =
+		u32x2{ pack2<T>(x[0] * inv, x[1] * inv),
+		       pack2<T>(x[2] * inv, x[3] * inv) };
+	if (a.lse && td == 0)
+		a.lse[row * c.heads + head] =
+			sum == 0.f ? -INFINITY :
+				     (unit + __builtin_amdgcn_logf(sum)) *
+					     0.693147181f;
+}
+
+template <typename T, int D>
+void join(const nvs_kv &c, const nvs_kv_attend_args &a, const nvs_plan &p,
+	  bool narrow, hipStream_t s)
+{
+	if (narrow)
+		hipLaunchKernelGGL((join_kernel<T, D, true>),
+				   dim3(c.batch * c.kv_heads * p.joined_rows),
+				   dim3(256), 0, s, c, a, p);
+	else
+		hipLaunchKernelGGL((join_kernel<T, D, false>),
+				   dim3(c.total * c.heads), dim3(256), 0, s, c,
+				   a, p);
+}
+
+} /* namespace */
+
+template <typename T, typename C>
+hipError_t nvs_wide(const nvs_kv &c, const nvs_kv_attend_args &a,
+		    const nvs_plan &p, hipStream_t s)
+{
+	const dim3 grid(p.wide_blocks * c.kv_heads * p.wide_parts);
+
+	if (c.dim == 64)
+		hipLaunchKernelGGL((wide_kernel<T, C, 64>), grid, dim3(256), 0,
+				   s, c, a, p);
+	else if (c.dim == 128)
+		hipLaunchKernelGGL((wide_kernel<T, C, 128>), grid, dim3(256),
+				   0, s, c, a, p);
+	else
+		hipLaunchKernelGGL((wide_kernel<T, C, 256>), grid, dim3(256),
+				   0, s, c, a, p);
+	return hipGetLastError();
+}
+
+template <typename T>
+hipError_t nvs_join(const nvs_kv &c, const nvs_kv_attend_args &a,
+		    const nvs_plan &p, bool narrow, hipStream_t s)
+{
+	if (c.dim == 64)
+		join<T, 64>(c, a, p, narrow, s);
+	else if (c.dim == 128)
+		join<T, 128>(c, a, p, narrow, s);
+	else
+		join<T, 256>(c, a, p, narrow, s);
+	return hipGetLastError();
+}
+
+#define INSTANCE(T, C)                                                     \
+	template hipError_t nvs_wide<T, C>(const nvs_kv &,                 \
+					   const nvs_kv_attend_args &,     \
+					   const nvs_plan &,               \
+					   hipStream_t);
+INSTANCE(bf16_t, bf16_t)
+INSTANCE(bf16_t, e4m3_t)
+INSTANCE(fp16_t, fp16_t)
+INSTANCE(fp16_t, e4m3_t)
+#define INSTANCE_JOIN(T)                                                   \
+	template hipError_t nvs_join<T>(const nvs_kv &,                    \
+					const nvs_kv_attend_args &,        \
+					const nvs_plan &, bool,            \
+					hipStream_t);
+INSTANCE_JOIN(bf16_t)
+INSTANCE_JOIN(fp16_t)

@@ -1,0 +1,329 @@
+/*
+ * nvshare-amd: what the attention kernels share.
+ *
+ * Rows and work.  The query heads of one cached head are rows of the same
+ * product: a sequence with n new tokens and G = heads / kv_heads has n * G
+ * rows for each cached head, row r being token r / G and head r % G.  Two
+ * kernels take blocks of these rows:
+ *
+ *   narrow  up to 32 rows, as single tokens and drafts have: its waves
+ *           share the rows and divide the keys, so that the cache streams
+ *           through all of them; bound by the cache's bytes
+ *   wide    128 rows, as chunks have: its waves divide the rows and share
+ *           the keys in LDS; bound by the matrix products
+ *
+ * Both walk the keys in tiles with the running maximum and sum of the
+ * softmax in 32 bits, and where there are few blocks of rows the keys are
+ * divided between `parts` blocks, whose results a third kernel joins in
+ * the order of the keys: no atomics, the same bits each time.
+ *
+ * Both compute S^T = K Q^T and O^T = V^T P^T, so that a lane has scores of
+ * one row only: maxima and sums need no more than an exchange between the
+ * wave's halves or quarters, and P^T is already laid out as the second
+ * product's operand.  V^T comes from LDS by transposing reads.
+ */
+#ifndef NVS_KVATTEND_H
+#define NVS_KVATTEND_H
+
+#include "kvdev.h"
+
+constexpr int NARROW_TILE = 32, WIDE_TILE = 64, WIDE_ROWS = 128;
+/* The fewest tiles that are worth a block of their own. */
+constexpr int NARROW_LEAST = 8, WIDE_LEAST = 8;
+
+/* How the work of one call is divided. */
+struct nvs_plan {
+	int narrow_rows; /* sequences with more rows go to the wide kernel */
+	int span;	 /* rows of a narrow block, 16 or 32 */
+	int joined_rows; /* rows of a sequence that narrow parts may have */
+	int narrow_parts, wide_parts; /* blocks that may divide the keys */
+	int wide_blocks;	      /* blocks of rows, for one cached head */
+	int page_shift; /* log2 of page_size, -1 where it is no power of 2 */
+	int cover; /* the launch that sees to rows of no sequence: 1 narrow,
+		      2 wide */
+	/* Results and (log2 of the weights' unit, sum of the weights in it)
+	 * of parts: [part][sequence][cached head][row of span] of narrow
+	 * blocks, [part][row][head] of wide ones. */
+	float *narrow_out, *wide_out;
+	f32x2 *narrow_sum, *wide_sum;
+};
+
+template <typename T, typename C>
+hipError_t nvs_narrow(const nvs_kv &c, const nvs_kv_attend_args &a,
+		      const nvs_plan &p, hipStream_t s);
+template <typename T, typename C>
+hipError_t nvs_wide(const nvs_kv &c, const nvs_kv_attend_args &a,
+		    const nvs_plan &p, hipStream_t s);
+template <typename T>
+hipError_t nvs_join(const nvs_kv &c, const nvs_kv_attend_args &a,
+		    const nvs_plan &p, bool narrow, hipStream_t s);
+
+/* The keys [lo, hi) that some of the tokens [i0, i1] of s see, and how many
+ * tiles of them a part has. */
+struct key_range {
+	int lo, hi;	 /* keys */
+	int first, last; /* tiles */
+	int per;	 /* tiles of a part */
+};
+
+__device__ __forceinline__ key_range keys_of(const nvs_kv &c, int window,
+					     const sequence &s, int i0, int i1,
+					     int tile, int least, int parts)
+{
+	const int64_t capacity = (int64_t)c.per_seq * c.page_size;
+	const int64_t hi = min(s.pos + i1 + 1, capacity);
+	const int64_t lo = window > 0 ? s.pos + i0 + 1 - window : 0;
+	key_range k;
+
+	k.lo = (int)min(max(lo, (int64_t)0), capacity);
+	k.hi = (int)max(hi, (int64_t)0);
+	if (k.hi <= k.lo) {
+		k.lo = k.hi = k.first = k.last = 0;
+		k.per = 1;
+		return k;
+	}
+	k.first = k.lo / tile;
+	k.last = (k.hi + tile - 1) / tile;
+	k.per = max(least, (k.last - k.first + parts - 1) / parts);
+	return k;
+}
+
+__device__ __forceinline__ int parts_of(const key_range &k)
+{
+	return max(1, (k.last - k.first + k.per - 1) / k.per);
+}
+
+/* Page and slot of a position. */
+__device__ __forceinline__ int entry_of(const nvs_kv &c, const nvs_plan &p,
+					int key)
+{
+	return p.page_shift >= 0 ? key >> p.page_shift : key / c.page_size;
+}
+
+__device__ __forceinline__ int slot_of(const nvs_kv &c, const nvs_plan &p,
+				       int key)
+{
+	return p.page_shift >= 0 ? key & (c.page_size - 1) :
+				   key % c.page_size;
+}
+
+/* The page of a key in [lo, hi); -1 for other keys and bad pages. */
+__device__ __forceinline__ int page_of(const nvs_kv &c, const nvs_plan &p,
+				       const int *table, int key,
+				       const key_range &k)
+{
+	if (key < k.lo || key >= k.hi)
+		return -1;
+	const int page = table[entry_of(c, p, key)];
+
+	return (unsigned)page < (unsigned)c.pages ? page : -1;
+}
+
+/* Read in the place of keys and values that are none: a value that is not
+ * seen still meets a weight of zero, so it has to be a finite number. */
+static __device__ const u32x4 no_value[32] = {};
+
+/* 16 bytes a lane from global memory to LDS, at `to` + 16 * lane; `to` is
+ * the same for the whole wave. */
+__device__ __forceinline__ void copy_to_lds(const char *from, char *to)
+{
+	__builtin_amdgcn_global_load_lds(
+		(const __attribute__((address_space(1))) void *)from,
+		(__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+
+/* At most N of the wave's loads still under way; no LDS access moves
+ * across. */
+template <int N> __device__ __forceinline__ void wait_loads()
+{
+	asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void wait_lds()
+{
+	asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
+/* Over the two halves (four quarters) of a wave. */
+__device__ __forceinline__ f32x2 halves(float x)
+{
+	const unsigned u = __builtin_bit_cast(unsigned, x);
+	const u32x2 r = __builtin_bit_cast(
+		u32x2, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+
+	return __builtin_bit_cast(f32x2, r);
+}
+
+__device__ __forceinline__ f32x2 odd_even_quarters(float x)
+{
+	const unsigned u = __builtin_bit_cast(unsigned, x);
+	const u32x2 r = __builtin_bit_cast(
+		u32x2, __builtin_amdgcn_permlane16_swap(u, u, false, false));
+
+	return __builtin_bit_cast(f32x2, r);
+}
+
+/*
+ * A row's running softmax.  Weights are exp2(s * c - unit) with c =
+ * scale * log2(e), unit = top * c - lift.  `top` follows the largest score
+ * only once that is `lag` powers of two ahead, so that the results are
+ * rescaled a few times and not with each tile; a weight then is at most
+ * 2^(lift + lag), which both types hold, and the sum is made of the same
+ * weights in 32 bits.
+ */
+template <typename T> struct softmax {
+	float top = -INFINITY, sum = 0.f;
+
+	__device__ __forceinline__ bool behind(float most, float c) const
+	{
+		return (most - top) * c > types<T>::lag ||
+		       (top == -INFINITY && most > top);
+	}
+
+	/* Follow the maximum; what the results so far are multiplied by. */
+	__device__ __forceinline__ float follow(float most, float c)
+	{
+		const float to = fmaxf(most, top);
+		const float keep = top == -INFINITY ?
+					   0.f :
+					   __builtin_amdgcn_exp2f((top - to) *
+								  c);
+		top = to;
+		sum *= keep;
+		return keep;
+	}
+
+	__device__ __forceinline__ float unit(float c) const
+	{
+		return top == -INFINITY ? 0.f : top * c - types<T>::lift;
+	}
+};
+
+/* The factor of a row's scores, and what its queries are multiplied by
+ * (as bits: a sign to flip, or all to clear) so that it is positive: the
+ * largest score then has the largest weight. */
+struct factor {
+	float c;
+	unsigned flip, keep;
+};
+
+__device__ __forceinline__ factor factor_of(float c)
+{
+	factor f = { fabsf(c), c < 0.f ? 0x80008000u : 0u, ~0u };
+
+	if (c == 0.f)
+		f = { 1.f, 0u, 0u };
+	return f;
+}
+
+/* Whether one of two numbers of type T (four e4m3) is infinite or NaN. */
+template <typename C> __device__ __forceinline__ bool not_finite(unsigned w)
+{
+	if constexpr (sizeof(C) == 1)
+		return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+	else
+		return ((w & types<C>::exponent) + types<C>::one) &
+		       0x80008000u;
+}
+
+/* A word of T (of e4m3) with zeros for what is infinite or NaN. */
+template <typename C> __device__ __forceinline__ unsigned finite_only(unsigned w)
+{
+	constexpr int BITS = 8 * sizeof(C);
+	constexpr unsigned FIELD = (1u << BITS) - 1u;
+
+#pragma unroll
+	for (int i = 0; i < 32; i += BITS)
+		if (not_finite<C>(w & (FIELD << i)))
+			w &= ~(FIELD << i);
+	return w;
+}
+
+/* x if it is infinite or NaN, else 0. */
+__device__ __forceinline__ float odd_only(float x)
+{
+	return __builtin_isfinite(x) ? 0.f : x;
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c)
+{
+	typedef typename types<T>::x8 x8;
+
+	if constexpr (__is_same(T, bf16_t))
+		return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+			__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b),
+			c, 0, 0, 0);
+	else
+		return __builtin_amdgcn_mfma_f32_16x16x32_f16(
+			__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b),
+			c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c)
+{
+	typedef typename types<T>::x8 x8;
+
+	if constexpr (__is_same(T, bf16_t))
+		return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+			__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b),
+			c, 0, 0, 0);
+	else
+		return __builtin_amdgcn_mfma_f32_32x32x16_f16(
+			__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b),
+			c, 0, 0, 0);
+}
+
+/* Four keys of one dimension a lane: of each 16 lanes, lane i gives the
+ * address of 4 dimensions of key i / 4 and gets dimension i of 4 keys. */
+__device__ __forceinline__ u32x2 read_keys4(const char *p)
+{
+	return __builtin_bit_cast(
+		u32x2,
+		__builtin_amdgcn_ds_read_tr16_b64_v4i16(
+			(__attribute__((address_space(3))) s16x4 *)p));
+}
+
+/* The same of 8 keys in e4m3: lane i gives 8 dimensions of key i / 2. */
+__device__ __forceinline__ u32x2 read_keys8(const char *p)
+{
+	typedef int s32x2 __attribute__((ext_vector_type(2)));
+
+	return __builtin_bit_cast(
+		u32x2,
+		__builtin_amdgcn_ds_read_tr8_b64_v2i32(
+			(__attribute__((address_space(3))) s32x2 *)p));
+}
+
+/* Rows that belong to no sequence: zeros where the buffer is the call's
+ * own, and -inf in any case; by the launch's blocks `who` of `many`. */
+template <typename T>
+__device__ __forceinline__ void cover_padding(const nvs_kv &c,
+					      const nvs_kv_attend_args &a,
+					      int64_t who, int64_t many)
+{
+	if (!c.starts)
+		return;
+	const int head = c.starts[0], tail = c.starts[c.batch];
+
+	for (int64_t row = who; row < c.total; row += many) {
+		if (row >= head && row < tail) {
+			/* On to this block's first row behind the last. */
+			row += (tail - row + many - 1) / many * many - many;
+			continue;
+		}
+		for (int i = threadIdx.x; i < c.heads * c.dim / 8;
+		     i += blockDim.x) {
+			const int h = i / (c.dim / 8), d = i % (c.dim / 8) * 8;
+
+			if (a.fill)
+				*(u32x4 *)((T *)a.out + row * a.out_row +
+					   h * a.out_head + d) = u32x4{};
+			if (a.lse && d == 0)
+				a.lse[row * c.heads + h] = -INFINITY;
+		}
+	}
+}
+
+#endif

@@ -45,6 +45,7 @@ struct nvs_kv_attend_args {
 	int window;  /* keys that a query sees, itself included; 0: all */
 	int max_new; /* no sequence has more rows than this */
 	int fill;
+	void *work; /* nvs_kv_attend_work() bytes */
 };
 
 #endif

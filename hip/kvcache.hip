@@ -17,64 +17,24 @@
  * outside [0, pages) is no page: nothing is stored in it and nothing of
  * it is attended to.
  */
-#include <hip/hip_runtime.h>
-
-#include <cstdint>
-
-#include "kvcache.h"
+#include "kvdev.h"
+#include "kvattend.h"
 
 namespace {
-
-typedef __bf16 bf16_t;
-typedef _Float16 fp16_t;
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-
-struct e4m3_t {
-	unsigned char bits;
-};
 
 template <typename T> struct vec8 {
 	T x[8];
 };
 
-__device__ __forceinline__ float to_f32(bf16_t x)
-{
-	return (float)x;
-}
-
-__device__ __forceinline__ float to_f32(fp16_t x)
-{
-	return (float)x;
-}
-
-__device__ __forceinline__ float to_f32(e4m3_t x)
-{
-	return __builtin_amdgcn_cvt_f32_fp8((int)x.bits, 0);
-}
-
-/* Eight values from 16 aligned bytes (8 of e4m3). */
+/* Eight values from 16 aligned bytes. */
 template <typename T>
 __device__ __forceinline__ void load8(const T *p, float *x)
 {
-	if constexpr (sizeof(T) == 1) {
-		u32x2 w = *(const u32x2 *)p;
+	const vec8<T> v = __builtin_bit_cast(vec8<T>, *(const u32x4 *)p);
+
 #pragma unroll
-		for (int i = 0; i < 2; i++) {
-			f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false);
-			f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
-			x[4 * i] = lo[0];
-			x[4 * i + 1] = lo[1];
-			x[4 * i + 2] = hi[0];
-			x[4 * i + 3] = hi[1];
-		}
-	} else {
-		vec8<T> v = __builtin_bit_cast(vec8<T>, *(const u32x4 *)p);
-#pragma unroll
-		for (int i = 0; i < 8; i++)
-			x[i] = (float)v.x[i];
-	}
+	for (int i = 0; i < 8; i++)
+		x[i] = (float)v.x[i];
 }
 
 /* Rounded to nearest, ties to even: the one rounding of each result. */
@@ -113,42 +73,6 @@ __device__ __forceinline__ void store8(e4m3_t *p, const float *x)
 	*(u32x2 *)p = w;
 }
 
-/* The place of a row: its sequence and position.  seq is -1 for a row
- * that belongs to no sequence (padding behind the last one). */
-struct place {
-	int seq;
-	int64_t pos;
-};
-
-__device__ __forceinline__ place place_of(const nvs_kv &c, int row)
-{
-	int first, count, b;
-
-	if (c.starts) {
-		/* The last b with starts[b] <= row. */
-		int lo = 0, hi = c.batch; /* in [lo, hi] */
-
-		while (lo < hi) {
-			int mid = (lo + hi + 1) >> 1;
-
-			if (c.starts[mid] <= row)
-				lo = mid;
-			else
-				hi = mid - 1;
-		}
-		if (lo == c.batch || c.starts[lo] > row)
-			return { -1, 0 };
-		b = lo;
-		first = c.starts[b];
-		count = c.starts[b + 1] - first;
-	} else {
-		count = c.total / c.batch;
-		b = row / count;
-		first = b * count;
-	}
-	return { b, (int64_t)c.lens[b] - count + (row - first) };
-}
-
 /* ------------------------------------------------------------------ */
 /* append                                                              */
 /* ------------------------------------------------------------------ */
@@ -178,9 +102,16 @@ __global__ __launch_bounds__(256) void append_kernel(nvs_kv c,
 	if (row64 >= c.total)
 		return;
 	const int row = (int)row64;
-	const place at = place_of(c, row);
-	const int64_t capacity = (int64_t)c.per_seq * c.page_size;
-	const bool in_range = at.seq >= 0 && at.pos >= 0 && at.pos < capacity;
+	const int b = sequence_at(c, row);
+	int64_t pos = -1;
+
+	if (b >= 0) {
+		const sequence s = sequence_of(c, b);
+
+		pos = s.pos + (row - s.first);
+	}
+	const int capacity = c.per_seq * c.page_size;
+	const bool in_range = pos >= 0 && pos < capacity;
 	const int kind = head < q_heads ? 0 :
 			 head < q_heads + c.kv_heads ? 1 : 2;
 	const int h = kind == 0 ? head : kind == 1 ? head - q_heads :
@@ -195,7 +126,7 @@ __global__ __launch_bounds__(256) void append_kernel(nvs_kv c,
 
 	if (!in_range) {
 		/* No token: queries give zeros in a buffer of our own. */
-		if (kind == 0 && (at.seq >= 0 || a.fill)) {
+		if (kind == 0 && (b >= 0 || a.fill)) {
 			float zero[8] = {};
 			T *o = (T *)a.q_out + row * a.q_out_row +
 			       h * a.q_out_head;
@@ -216,7 +147,7 @@ __global__ __launch_bounds__(256) void append_kernel(nvs_kv c,
 	load8(src + e0, x0);
 	load8(src + e1, x1);
 	if (turn) {
-		const float *cs = a.rotation + at.pos * a.rotation_row + 8 * u;
+		const float *cs = a.rotation + pos * a.rotation_row + 8 * u;
 		const float *sn = cs + a.rotary / 2;
 
 		if (a.interleaved) {
@@ -246,9 +177,9 @@ __global__ __launch_bounds__(256) void append_kernel(nvs_kv c,
 		return;
 	}
 
-	const int entry = (int)(at.pos / c.page_size);
-	const int slot = (int)(at.pos % c.page_size);
-	const int page = c.table[at.seq * c.table_row + entry];
+	const int entry = (int)(pos / c.page_size);
+	const int slot = (int)(pos % c.page_size);
+	const int page = c.table[b * c.table_row + entry];
 
 	if ((unsigned)page >= (unsigned)c.pages)
 		return;
@@ -271,108 +202,6 @@ __global__ __launch_bounds__(256) void append_kernel(nvs_kv c,
 	store8(dst + e1, x1);
 }
 
-/* ------------------------------------------------------------------ */
-/* attend                                                              */
-/* ------------------------------------------------------------------ */
-
-/*
- * One wave to a query row and head, 64 keys at a time with the running
- * maximum and sum of the softmax in 32 bits: a lane has a key while the
- * scores are made, and dimensions while the values are added.
- */
-template <typename T, typename C>
-__global__ __launch_bounds__(64) void attend_kernel(nvs_kv c, nvs_kv_attend_args a)
-{
-	__shared__ float q[256], p[64];
-	__shared__ int64_t where[64];
-	const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-	const int kh = h / (c.heads / c.kv_heads);
-	const place at = place_of(c, row);
-	T *out = (T *)a.out + row * a.out_row + h * a.out_head;
-
-	if (at.seq < 0) {
-		if (a.fill)
-			for (int d = lane; d < c.dim; d += 64)
-				out[d] = (T)0.f;
-		if (a.lse && lane == 0)
-			a.lse[(int64_t)row * c.heads + h] = -INFINITY;
-		return;
-	}
-	const int64_t capacity = (int64_t)c.per_seq * c.page_size;
-	const int64_t end = min(at.pos + 1, capacity);
-	const int64_t begin = a.window > 0 && at.pos + 1 > a.window ?
-				      at.pos + 1 - a.window : 0;
-	const T *src = (const T *)a.q + row * a.q_row + h * a.q_head;
-	const float ks = c.k_scale ? c.k_scale[kh] : 1.f;
-	const float vs = c.v_scale ? c.v_scale[kh] : 1.f;
-	float top = -INFINITY, sum = 0.f, acc[4] = {};
-
-	for (int d = lane; d < c.dim; d += 64)
-		q[d] = to_f32(src[d]) * a.scale * ks;
-	__syncthreads();
-	for (int64_t j0 = begin; j0 < end; j0 += 64) {
-		const int64_t j = j0 + lane;
-		float s = -INFINITY;
-		int page = -1;
-
-		if (j < end)
-			page = c.table[at.seq * c.table_row + j / c.page_size];
-		const bool seen = (unsigned)page < (unsigned)c.pages;
-		const int64_t slot = j % c.page_size;
-
-		where[lane] = -1;
-		if (seen) {
-			const C *k = (const C *)c.k_cache + page * c.k_page +
-				     slot * c.k_slot + kh * c.k_head;
-
-			s = 0.f;
-			for (int d = 0; d < c.dim; d += 8) {
-				float x[8];
-
-				load8(k + d, x);
-				for (int i = 0; i < 8; i++)
-					s += q[d + i] * x[i];
-			}
-			where[lane] = page * c.v_page + slot * c.v_slot +
-				      kh * c.v_head;
-		}
-		float m = s;
-		for (int o = 32; o; o >>= 1)
-			m = fmaxf(m, __shfl_xor(m, o));
-		m = fmaxf(m, top);
-		const float base = m == -INFINITY ? 0.f : m;
-		const float e = seen ? expf(s - base) : 0.f;
-		const float keep = expf(top - base);
-		float t = e;
-		for (int o = 32; o; o >>= 1)
-			t += __shfl_xor(t, o);
-		sum = sum * keep + t;
-		top = m;
-		p[lane] = e;
-		__syncthreads();
-		for (int i = 0; i < 4; i++)
-			acc[i] *= keep;
-		for (int n = 0; n < 64; n++) {
-			if (where[n] < 0)
-				continue;
-			const C *v = (const C *)c.v_cache + where[n];
-
-			for (int i = 0; i < 4; i++)
-				if (lane + 64 * i < c.dim)
-					acc[i] += p[n] *
-						  to_f32(v[lane + 64 * i]);
-		}
-		__syncthreads();
-	}
-	for (int i = 0; i < 4; i++)
-		if (lane + 64 * i < c.dim)
-			out[lane + 64 * i] =
-				(T)(sum == 0.f ? 0.f : acc[i] / sum * vs);
-	if (a.lse && lane == 0)
-		a.lse[(int64_t)row * c.heads + h] =
-			sum == 0.f ? -INFINITY : top + logf(sum);
-}
-
 bool aligned(const void *p, int64_t bytes)
 {
 	return ((uintptr_t)p & (bytes - 1)) == 0;
@@ -387,6 +216,8 @@ bool sound(const nvs_kv &c)
 
 	return c.batch > 0 && c.total >= 0 && c.heads > 0 && c.kv_heads > 0 &&
 	       c.heads % c.kv_heads == 0 && c.pages > 0 && c.page_size > 0 &&
+	       (int64_t)c.total * c.heads < 0x7fffffff &&
+	       (int64_t)c.per_seq * c.page_size <= 0x7fffffff &&
 	       c.per_seq > 0 && c.k_cache && c.v_cache && c.lens && c.table &&
 	       (c.type == NVS_KV_BF16 || c.type == NVS_KV_FP16) &&
 	       (c.cache_type == c.type || c.cache_type == NVS_KV_E4M3) &&
@@ -396,23 +227,117 @@ bool sound(const nvs_kv &c)
 	       aligned(c.v_cache, 16);
 }
 
+/* A grid's threads are counted in 32 bits. */
+bool too_large(int64_t blocks, int64_t threads)
+{
+	return blocks * threads > 0xffffffffll;
+}
+
 template <typename T, typename C>
 int launch_append(const nvs_kv &c, const nvs_kv_append_args &a, hipStream_t s)
 {
 	const int64_t all = (a.q ? c.heads : 0) + 2 * c.kv_heads;
 	const int64_t n = c.total * all * (c.dim / 16);
 
+	if (too_large((n + 255) / 256, 256))
+		return (int)hipErrorInvalidValue;
 	hipLaunchKernelGGL((append_kernel<T, C>), dim3((n + 255) / 256),
 			   dim3(256), 0, s, c, a);
 	return (int)hipGetLastError();
 }
 
-template <typename T, typename C>
-int launch_attend(const nvs_kv &c, const nvs_kv_attend_args &a, hipStream_t s)
+bool sound_attend(const nvs_kv &c, const nvs_kv_attend_args &a)
 {
-	hipLaunchKernelGGL((attend_kernel<T, C>), dim3(c.total, c.heads),
-			   dim3(64), 0, s, c, a);
-	return (int)hipGetLastError();
+	return (c.dim == 64 || c.dim == 128 || c.dim == 256) && a.q && a.out &&
+	       a.window >= 0 && a.max_new >= 0 &&
+	       (a.q_row | a.q_head | a.out_row | a.out_head) % 8 == 0 &&
+	       aligned(a.q, 16) && aligned(a.out, 16);
+}
+
+int64_t ceil_div(int64_t a, int64_t b)
+{
+	return (a + b - 1) / b;
+}
+
+/*
+ * The division of a call's work, by what the host knows: rows, sequences,
+ * the table's width and the most rows that a sequence may have.  With few
+ * blocks of rows, the keys are divided so that there are enough blocks for
+ * 256 CUs to be evenly loaded.
+ */
+nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, int64_t &bytes)
+{
+	const int64_t group = c.heads / c.kv_heads;
+	const int64_t most_new = c.starts ? a.max_new : c.total / c.batch;
+	const int64_t most_rows = most_new * group;
+	int64_t keys = (int64_t)c.per_seq * c.page_size;
+	nvs_plan p = {};
+
+	if (a.window > 0)
+		keys = keys < a.window + most_new ? keys : a.window + most_new;
+	p.page_shift = c.page_size & (c.page_size - 1) ?
+			       -1 :
+			       __builtin_ctz(c.page_size);
+	p.span = most_rows > 32 || most_rows <= 16 ? 16 : 32;
+	p.narrow_rows = most_rows <= 32 ? 0x7fffffff : c.starts ? 16 : 0;
+	p.joined_rows = (int)(most_rows < p.span ? most_rows : p.span);
+	p.narrow_parts = p.wide_parts = 1;
+	if (p.narrow_rows && p.joined_rows) {
+		const int64_t items = (int64_t)c.batch * c.kv_heads;
+		const int64_t want = ceil_div(1024, items);
+		const int64_t most =
+			ceil_div(ceil_div(keys, NARROW_TILE), NARROW_LEAST);
+
+		p.narrow_parts = (int)(want < most ? want : most);
+	}
+	if (most_rows > 32) {
+		p.wide_blocks =
+			(int)(c.starts ? c.total * group / WIDE_ROWS + c.batch :
+					 c.batch *
+						 ceil_div(most_rows, WIDE_ROWS));
+		const int64_t want = 512 / ((int64_t)p.wide_blocks *
+					    c.kv_heads);
+		const int64_t most =
+			ceil_div(ceil_div(keys, WIDE_TILE), WIDE_LEAST);
+
+		p.wide_parts = (int)(want < 1 ? 1 : want < most ? want : most);
+	}
+	if (c.starts)
+		p.cover = p.narrow_rows ? 1 : 2;
+
+	/* The parts' results, narrow before wide. */
+	char *work = (char *)a.work;
+	const int64_t narrow = p.narrow_parts > 1 ?
+				       (int64_t)p.narrow_parts * c.batch *
+					       c.kv_heads * p.span :
+				       0;
+	const int64_t wide = p.wide_parts > 1 ? (int64_t)p.wide_parts *
+							c.total * c.heads :
+						0;
+
+	p.narrow_out = (float *)work;
+	p.wide_out = p.narrow_out + narrow * c.dim;
+	p.narrow_sum = (f32x2 *)(p.wide_out + wide * c.dim);
+	p.wide_sum = p.narrow_sum + narrow;
+	bytes = (narrow + wide) * (c.dim * 4 + 8);
+	return p;
+}
+
+template <typename T, typename C>
+int launch_attend(const nvs_kv &c, const nvs_kv_attend_args &a,
+		  const nvs_plan &p, hipStream_t s)
+{
+	hipError_t e = hipSuccess;
+
+	if (p.narrow_rows)
+		e = nvs_narrow<T, C>(c, a, p, s);
+	if (e == hipSuccess && p.wide_blocks)
+		e = nvs_wide<T, C>(c, a, p, s);
+	if (e == hipSuccess && p.narrow_parts > 1)
+		e = nvs_join<T>(c, a, p, true, s);
+	if (e == hipSuccess && p.wide_parts > 1)
+		e = nvs_join<T>(c, a, p, false, s);
+	return (int)e;
 }
 
 } /* namespace */
@@ -447,18 +372,35 @@ int nvs_kv_append(const nvs_kv *c, const nvs_kv_append_args *a, void *stream)
 	return BY_TYPE(launch_append, *c, *a, (hipStream_t)stream);
 }
 
+/* Bytes that nvs_kv_attend needs at args.work; -1: refused. */
+int64_t nvs_kv_attend_work(const nvs_kv *c, const nvs_kv_attend_args *a)
+{
+	int64_t bytes;
+
+	if (!c || !a || !sound(*c) || !sound_attend(*c, *a))
+		return -1;
+	if (c->total == 0)
+		return 0;
+	plan_of(*c, *a, bytes);
+	return bytes;
+}
+
 int nvs_kv_attend(const nvs_kv *c, const nvs_kv_attend_args *a, void *stream)
 {
-	if (!c || !a || !sound(*c) ||
-	    (c->dim != 64 && c->dim != 128 && c->dim != 256) || !a->q ||
-	    !a->out || a->window < 0)
-		return (int)hipErrorInvalidValue;
-	if ((a->q_row | a->q_head | a->out_row | a->out_head) % 8 ||
-	    !aligned(a->q, 16) || !aligned(a->out, 16))
+	int64_t bytes;
+
+	if (!c || !a || !sound(*c) || !sound_attend(*c, *a))
 		return (int)hipErrorInvalidValue;
 	if (c->total == 0)
 		return 0;
-	return BY_TYPE(launch_attend, *c, *a, (hipStream_t)stream);
+	const nvs_plan p = plan_of(*c, *a, bytes);
+
+	if ((bytes && (!a->work || !aligned(a->work, 16))) ||
+	    too_large((int64_t)c->batch * c->kv_heads * p.narrow_parts, 256) ||
+	    too_large((int64_t)p.wide_blocks * c->kv_heads * p.wide_parts,
+		      256))
+		return (int)hipErrorInvalidValue;
+	return BY_TYPE(launch_attend, *c, *a, p, (hipStream_t)stream);
 }
 
 } /* extern "C" */

@@ -48,7 +48,7 @@ class KvAttend(ctypes.Structure):
 
     _fields_ = _fields(
         "ptr: q out lse; i64: q_row q_head out_row out_head;"
-        "f32: scale; int: window max_new fill")
+        "f32: scale; int: window max_new fill; ptr: work")
 
 
 KV_BF16, KV_FP16, KV_E4M3 = 0, 1, 2
@@ -129,6 +129,13 @@ class HipUtil:
                                         ctypes.c_void_p(stream)),
                  "kv_append")
 
+    def kv_attend_work(self, cache: KvCache, args: KvAttend) -> int:
+        """Bytes that kv_attend needs at args.work."""
+        n = self.lib.nvs_kv_attend_work(ctypes.byref(cache),
+                                        ctypes.byref(args))
+        self._ck(1 if n < 0 else 0, "kv_attend_work")
+        return n
+
     def kv_attend(self, cache: KvCache, args: KvAttend,
                   stream: int) -> None:
         self._ck(self.lib.nvs_kv_attend(ctypes.byref(cache),
@@ -162,4 +169,5 @@ def load() -> HipUtil:
                   "nvs_hip_mem_get_info", "nvs_kv_append",
                   "nvs_kv_attend"):
         getattr(lib, fname).restype = ctypes.c_int
+    lib.nvs_kv_attend_work.restype = ctypes.c_int64
     return HipUtil(lib)

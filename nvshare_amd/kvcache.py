@@ -195,6 +195,8 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor,
         raise ValueError(f"dim {dim} is not one of {ATTEND_DIMS}")
     if scale is None:
         scale = dim ** -0.5
+    elif not math.isfinite(scale):
+        raise ValueError(f"scale {scale} is not finite")
     if window is None:
         window = 0
     elif window < 1:
@@ -230,7 +232,11 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor,
     args = hiputil.KvAttend(
         q.data_ptr(), out.data_ptr(),
         lse.data_ptr() if lse is not None else None, *q.stride()[:2],
-        *out.stride()[:2], scale, window, min(max_new, total), int(fill))
+        *out.stride()[:2], scale, window, min(max_new, total), int(fill), None)
+    size = _lib().kv_attend_work(kv, args)
+    if size:
+        work = torch.empty(size, dtype=torch.uint8, device=q.device)
+        args.work = work.data_ptr()
     _launch(q, _lib().kv_attend, kv, args)
     return result
 
@@ -245,8 +251,9 @@ def _rows(name: str, t: torch.Tensor) -> tuple[int, int, int]:
     if t.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"{name}: bfloat16 or float16 is wanted, got "
                          f"{t.dtype}")
-    if t.shape[0] > 2**31 - 1:
-        raise ValueError(f"{name}: {t.shape[0]} rows pass 31 bits")
+    if t.shape[0] * t.shape[1] >= 2**31 - 1:
+        raise ValueError(f"{name}: {t.shape[0]} rows of {t.shape[1]} heads "
+                         "pass 31 bits")
     return t.shape
 
 

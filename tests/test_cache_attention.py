@@ -835,6 +835,7 @@ def test_refusals(device):
                                       for x in cache[:2])),
                        q=q[..., :48].contiguous()))
     refused("window", att(window=0))
+    refused("scale", att(scale=math.nan))
     refused("max_new", att(max_new=-1, starts=starts))
     refused("out", att(out=q[:2]))
     refused("out", att(out=q.float()))
@@ -905,7 +906,7 @@ def test_structures_match_the_header():
     text = (REPO_ROOT / "hip" / "kvcache.h").read_text()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     kinds = {"int64_t": hiputil.ctypes.c_int64, "int": hiputil.ctypes.c_int,
-             "float": hiputil.ctypes.c_float}
+             "float": hiputil.ctypes.c_float}  # and pointers
     for struct, cls in (("nvs_kv", hiputil.KvCache),
                         ("nvs_kv_append_args", hiputil.KvAppend),
                         ("nvs_kv_attend_args", hiputil.KvAttend)):
