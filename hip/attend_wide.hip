@@ -503,98 +503,132 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 }
 
 /*
- * Join the parts of rows whose keys were divided: a block to a row, its
- * threads over the dimensions and then over the parts.  Rows with one part
- * have their result already.
+ * Join the parts of rows whose keys were divided.  Rows with one part have
+ * their result already.  A row has 256 / ROWS threads: first over the
+ * parts, for their weights, then over the dimensions and TP parts at a
+ * time.  With many parts a whole block is at work on a row, so that their
+ * loads are under way together; with few, a wave is.
  */
-template <typename T, int D, bool NARROW>
+template <typename T, int D, bool NARROW, int ROWS>
 __global__ __launch_bounds__(256) void join_kernel(nvs_kv c,
 						   nvs_kv_attend_args a,
-						   nvs_plan p)
+						   nvs_plan p, int all_rows)
 {
-	constexpr int TD = D / 4, TP = 256 / TD; /* threads: dims, parts */
-	__shared__ f32x4 add[TP][TD];
-	__shared__ float adds[TP];
-	const int td = threadIdx.x % TD, tp = threadIdx.x / TD;
+	constexpr int THREADS = 256 / ROWS;
+	constexpr int PER = ROWS == 1 ? 4 : D / 64 > 4 ? 4 : D / 64;
+	constexpr int TD = D / PER, TP = THREADS / TD;
+	constexpr int MOST = ROWS == 1 ? JOIN_MOST : JOIN_FEW;
+	typedef float vec __attribute__((ext_vector_type(PER)));
+	__shared__ vec add[ROWS][TP][TD];
+	__shared__ float scales[ROWS][MOST];
+	const int sub = threadIdx.x / THREADS, t = threadIdx.x % THREADS;
+	const int td = t % TD, tp = t / TD;
 	const int group = c.heads / c.kv_heads;
-	int b, r, head;
+	const int index = blockIdx.x * ROWS + sub;
+	bool mine = index < all_rows;
+	int b = 0, r = 0, head = 0, rows = 0;
+	int64_t at = 0, step = 0; /* of the row in a part, between parts */
+	sequence s = {};
 
-	if (NARROW) {
-		const int item = blockIdx.x / p.joined_rows;
+	if (mine) {
+		if (NARROW) {
+			const int item = index / p.joined_rows;
 
-		b = item / c.kv_heads;
-		r = blockIdx.x % p.joined_rows;
-		head = item % c.kv_heads * group + r % group;
-	} else {
-		head = blockIdx.x % c.heads;
-		b = sequence_at(c, blockIdx.x / c.heads);
-		if (b < 0)
-			return;
+			b = item / c.kv_heads;
+			r = index % p.joined_rows;
+			head = item % c.kv_heads * group + r % group;
+			s = sequence_of(c, b);
+			rows = s.count * group;
+			mine = r < rows && rows <= p.joined_rows;
+			at = (int64_t)item * p.span + r;
+			step = (int64_t)c.batch * c.kv_heads * p.span;
+		} else {
+			head = index % c.heads;
+			b = sequence_at(c, index / c.heads);
+			mine = b >= 0;
+			if (mine) {
+				s = sequence_of(c, b);
+				rows = s.count * group;
+				r = (index / c.heads - s.first) * group +
+				    head % group;
+				mine = r < rows && rows > p.narrow_rows;
+			}
+			at = index;
+			step = (int64_t)c.total * c.heads;
+		}
 	}
-	const sequence s = sequence_of(c, b);
-	const int rows = s.count * group, kh = head / group;
-	int64_t at, step; /* of the row in a part, and between parts */
+	int parts = 1;
 
-	if (NARROW) {
-		if (r >= rows || rows > p.joined_rows)
-			return;
-		at = ((int64_t)b * c.kv_heads + kh) * p.span + r;
-		step = (int64_t)c.batch * c.kv_heads * p.span;
-	} else {
-		r = ((int)(blockIdx.x / c.heads) - s.first) * group +
-		    head % group;
-		if (r >= rows || rows <= p.narrow_rows)
-			return;
-		at = blockIdx.x;
-		step = (int64_t)c.total * c.heads;
+	if (mine) {
+		const int span = NARROW ? p.span : WIDE_ROWS;
+		const int r0 = r / span * span;
+
+		parts = parts_of(keys_of(
+			c, a.window, s, r0 / group,
+			min(s.count, (r0 + span - 1) / group + 1) - 1,
+			NARROW ? NARROW_TILE : WIDE_TILE,
+			NARROW ? NARROW_LEAST : WIDE_LEAST,
+			NARROW ? p.narrow_parts : p.wide_parts));
+		mine = parts > 1;
 	}
-	const int span = NARROW ? p.span : WIDE_ROWS;
-	const int r0 = r / span * span;
-	const key_range k = keys_of(
-		c, a.window, s, r0 / group,
-		min(s.count, (r0 + span - 1) / group + 1) - 1,
-		NARROW ? NARROW_TILE : WIDE_TILE,
-		NARROW ? NARROW_LEAST : WIDE_LEAST,
-		NARROW ? p.narrow_parts : p.wide_parts);
-	const int parts = parts_of(k);
-
-	if (parts < 2)
+	if (ROWS == 1 && !mine)
 		return;
 	const f32x2 *sums = (NARROW ? p.narrow_sum : p.wide_sum) + at;
 	const float *outs = (NARROW ? p.narrow_out : p.wide_out) + at * D +
-			    4 * td;
-	float unit = -INFINITY, sum = 0.f;
-	f32x4 x = {};
+			    PER * td;
 
-	for (int n = 0; n < parts; n++)
-		unit = fmaxf(unit, sums[n * step][0]);
-	for (int n = tp; n < parts; n += TP) {
-		const f32x2 y = sums[n * step];
-		const float m = y[0] == -INFINITY ?
+	/* The parts' weights, by the first wave of the row's threads. */
+	float unit = -INFINITY, sum = 0.f;
+
+	if (mine && t < 64) {
+		for (int n = t; n < parts; n += 64)
+			unit = fmaxf(unit, sums[n * step][0]);
+		for (int o = 32; o; o >>= 1)
+			unit = fmaxf(unit, __shfl_xor(unit, o));
+		for (int n = t; n < parts; n += 64) {
+			const f32x2 y = sums[n * step];
+			const float m =
+				y[0] == -INFINITY ?
 					0.f :
 					__builtin_amdgcn_exp2f(y[0] - unit);
 
-		sum += m * y[1];
-		x += m * *(const f32x4 *)(outs + n * step * D);
+			scales[sub][n] = m;
+			sum += m * y[1];
+		}
+		for (int o = 32; o; o >>= 1)
+			sum += __shfl_xor(sum, o);
 	}
-	add[tp][td] = x;
-	if (td == 0)
-		adds[tp] = sum;
 	__syncthreads();
-	if (tp)
-		return;
-	sum = adds[0];
-	for (int n = 1; n < TP; n++) {
-		x += add[n][td];
-		sum += adds[n];
+	vec x = {};
+
+	if (mine) {
+#pragma unroll 8
+		for (int n = tp; n < parts; n += TP)
+			x += scales[sub][n] * *(const vec *)(outs + n * step * D);
 	}
+	if (TP > 1) {
+		add[sub][tp][td] = x;
+		__syncthreads();
+		if (tp == 0)
+			for (int n = 1; n < TP; n++)
+				x += add[sub][n][td];
+		/* `sum` is the first wave's: TD is at most that. */
+	}
+	if (!mine || tp)
+		return;
+	const int kh = head / group;
 	const float inv =
 		sum == 0.f ? 0.f : (c.v_scale ? c.v_scale[kh] : 1.f) / sum;
 	const int64_t row = s.first + r / group;
+	T *o = (T *)a.out + row * a.out_row + head * a.out_head + PER * td;
 
-	*(u32x2 *)((T *)a.out + row * a.out_row + head * a.out_head + 4 * td) =
-		u32x2{ pack2<T>(x[0] * inv, x[1] * inv),
-		       pack2<T>(x[2] * inv, x[3] * inv) };
+	if constexpr (PER == 1)
+		*o = (T)(x[0] * inv);
+	else
+#pragma unroll
+		for (int e = 0; e < PER; e += 2)
+			*(unsigned *)(o + e) =
+				pack2<T>(x[e] * inv, x[e + 1] * inv);
 	if (a.lse && td == 0)
 		a.lse[row * c.heads + head] =
 			sum == 0.f ? -INFINITY :
@@ -602,18 +636,20 @@ __global__ __launch_bounds__(256) void join_kernel(nvs_kv c,
 					     0.693147181f;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool NARROW>
 void join(const nvs_kv &c, const nvs_kv_attend_args &a, const nvs_plan &p,
-	  bool narrow, hipStream_t s)
+	  hipStream_t s)
 {
-	if (narrow)
-		hipLaunchKernelGGL((join_kernel<T, D, true>),
-				   dim3(c.batch * c.kv_heads * p.joined_rows),
-				   dim3(256), 0, s, c, a, p);
+	const int rows = NARROW ? c.batch * c.kv_heads * p.joined_rows :
+				  c.total * c.heads;
+
+	if ((NARROW ? p.narrow_parts : p.wide_parts) > JOIN_FEW)
+		hipLaunchKernelGGL((join_kernel<T, D, NARROW, 1>), dim3(rows),
+				   dim3(256), 0, s, c, a, p, rows);
 	else
-		hipLaunchKernelGGL((join_kernel<T, D, false>),
-				   dim3(c.total * c.heads), dim3(256), 0, s, c,
-				   a, p);
+		hipLaunchKernelGGL((join_kernel<T, D, NARROW, 4>),
+				   dim3((rows + 3) / 4), dim3(256), 0, s, c, a,
+				   p, rows);
 }
 
 } /* namespace */
@@ -641,11 +677,14 @@ hipError_t nvs_join(const nvs_kv &c, const nvs_kv_attend_args &a,
 		    const nvs_plan &p, bool narrow, hipStream_t s)
 {
 	if (c.dim == 64)
-		join<T, 64>(c, a, p, narrow, s);
+		narrow ? join<T, 64, true>(c, a, p, s) :
+			 join<T, 64, false>(c, a, p, s);
 	else if (c.dim == 128)
-		join<T, 128>(c, a, p, narrow, s);
+		narrow ? join<T, 128, true>(c, a, p, s) :
+			 join<T, 128, false>(c, a, p, s);
 	else
-		join<T, 256>(c, a, p, narrow, s);
+		narrow ? join<T, 256, true>(c, a, p, s) :
+			 join<T, 256, false>(c, a, p, s);
 	return hipGetLastError();
 }
 

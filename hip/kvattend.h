@@ -31,6 +31,9 @@ constexpr int NARROW_TILE = 32, WIDE_TILE = 64, WIDE_ROWS = 128;
 /* The fewest tiles that are worth a block of their own. */
 constexpr int NARROW_LEAST = 8, WIDE_LEAST = 8;
 
+/* The most parts, and the most that one wave joins. */
+constexpr int JOIN_MOST = 1024, JOIN_FEW = 16;
+
 /* How the work of one call is divided. */
 struct nvs_plan {
 	int narrow_rows; /* sequences with more rows go to the wide kernel */

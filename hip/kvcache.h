@@ -1,7 +1,7 @@
 /*
  * nvshare-amd: arguments of the paged key/value cache's kernels
- * (libnvshare_hiputil.so).  nvshare_amd/hiputil.py holds the same
- * structures.  Strides are in values, not bytes.
+ * (libnvshare_hiputil.so).  nvshare_amd/hiputil.py lays them out by the
+ * same members.  Strides are in values, not bytes.
  */
 #ifndef NVS_KVCACHE_H
 #define NVS_KVCACHE_H
@@ -45,7 +45,6 @@ struct nvs_kv_attend_args {
 	int window;  /* keys that a query sees, itself included; 0: all */
 	int max_new; /* no sequence has more rows than this */
 	int fill;
-	void *work; /* nvs_kv_attend_work() bytes */
 };
 
 #endif

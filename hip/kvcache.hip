@@ -265,7 +265,8 @@ int64_t ceil_div(int64_t a, int64_t b)
  * blocks of rows, the keys are divided so that there are enough blocks for
  * 256 CUs to be evenly loaded.
  */
-nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, int64_t &bytes)
+nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, void *work,
+		 int64_t &bytes)
 {
 	const int64_t group = c.heads / c.kv_heads;
 	const int64_t most_new = c.starts ? a.max_new : c.total / c.batch;
@@ -306,7 +307,6 @@ nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, int64_t &bytes)
 		p.cover = p.narrow_rows ? 1 : 2;
 
 	/* The parts' results, narrow before wide. */
-	char *work = (char *)a.work;
 	const int64_t narrow = p.narrow_parts > 1 ?
 				       (int64_t)p.narrow_parts * c.batch *
 					       c.kv_heads * p.span :
@@ -372,7 +372,7 @@ int nvs_kv_append(const nvs_kv *c, const nvs_kv_append_args *a, void *stream)
 	return BY_TYPE(launch_append, *c, *a, (hipStream_t)stream);
 }
 
-/* Bytes that nvs_kv_attend needs at args.work; -1: refused. */
+/* Bytes that nvs_kv_attend needs at `work`; -1: refused. */
 int64_t nvs_kv_attend_work(const nvs_kv *c, const nvs_kv_attend_args *a)
 {
 	int64_t bytes;
@@ -381,11 +381,12 @@ int64_t nvs_kv_attend_work(const nvs_kv *c, const nvs_kv_attend_args *a)
 		return -1;
 	if (c->total == 0)
 		return 0;
-	plan_of(*c, *a, bytes);
+	plan_of(*c, *a, nullptr, bytes);
 	return bytes;
 }
 
-int nvs_kv_attend(const nvs_kv *c, const nvs_kv_attend_args *a, void *stream)
+int nvs_kv_attend(const nvs_kv *c, const nvs_kv_attend_args *a, void *work,
+		  void *stream)
 {
 	int64_t bytes;
 
@@ -393,9 +394,9 @@ int nvs_kv_attend(const nvs_kv *c, const nvs_kv_attend_args *a, void *stream)
 		return (int)hipErrorInvalidValue;
 	if (c->total == 0)
 		return 0;
-	const nvs_plan p = plan_of(*c, *a, bytes);
+	const nvs_plan p = plan_of(*c, *a, work, bytes);
 
-	if ((bytes && (!a->work || !aligned(a->work, 16))) ||
+	if ((bytes && (!work || !aligned(work, 16))) ||
 	    too_large((int64_t)c->batch * c->kv_heads * p.narrow_parts, 256) ||
 	    too_large((int64_t)p.wide_blocks * c->kv_heads * p.wide_parts,
 		      256))

@@ -56,6 +56,7 @@ from nvshare_amd import hiputil
 E4M3_MAX = 448.0
 ATTEND_DIMS = (64, 128, 256)
 
+_ROW_TYPES = (torch.bfloat16, torch.float16)
 _TYPES = {torch.bfloat16: hiputil.KV_BF16, torch.float16: hiputil.KV_FP16,
           torch.float8_e4m3fn: hiputil.KV_E4M3}
 
@@ -113,38 +114,25 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor,
     `q` [total, heads, dim] gives a new tensor, or goes into `q_out`, which
     may be q itself.  Rows of no sequence are zero in a new tensor and left
     as they are in `q_out`; rows without a place in the table are zero."""
+    total, _, dim = _rows("k", k)
     _like("v", v, k)
-    if q is None and q_out is not None:
-        raise ValueError("q_out without q")
-    total, kv_heads, dim = _rows("k", k)
-    heads = kv_heads
+    heads = k.shape[1]
     if q is not None:
         _like("q", q, k, heads=True)
         heads = q.shape[1]
-    kv = _describe(cache, k, heads, table, lens, starts)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    batch, per_seq = _check(cache, k, heads, table, lens, starts)
     if dim % 16:
         raise ValueError(f"dim {dim} is no multiple of 16")
-    rotary = 0
     if rotation is not None:
-        rotary = rotation.shape[-1]
-        if (rotation.dim() != 2 or rotation.dtype != torch.float32
-                or rotation.get_device() != k.get_device()):
-            raise ValueError("rotation: a float32 [positions, rotary] "
-                             "tensor on the device of k is wanted")
-        if rotary == 0 or rotary % 16 or rotary > dim:
-            raise ValueError(f"rotation: {rotary} dimensions are no "
-                             f"multiple of 16 up to {dim}")
-        if rotation.shape[0] < kv.per_seq * kv.page_size:
-            raise ValueError(f"rotation: {rotation.shape[0]} positions, the "
-                             f"table names {kv.per_seq * kv.page_size}")
+        _check_rotation(rotation, k, per_seq * cache.k.shape[1])
     fill = q_out is None
     if q is not None:
         if fill:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = q.new_empty(q.shape)
         else:
-            _like("q_out", q_out, q, heads=True)
-            if q_out.shape != q.shape:
-                raise ValueError("q_out is not shaped as q")
+            _like("q_out", q_out, q)
     _forward_only(k, v, q)
     if total == 0:
         return q_out
@@ -152,22 +140,26 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor,
         _append_plain(cache, k, v, table, lens, starts, q, rotation,
                       interleaved, q_out, fill)
         return q_out
-    for name, t in (("k", k), ("v", v), ("q", q), ("q_out", q_out)):
-        if t is not None:
-            _strides(name, t, 8)
-    if rotation is not None and (rotation.stride(1) != 1
-                                 or rotation.stride(0) % 4
-                                 or rotation.data_ptr() % 16):
-        raise ValueError("rotation: rows are not contiguous at 16 bytes")
-    args = hiputil.KvAppend(
-        q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(),
-        q_out.data_ptr() if q is not None else None,
-        rotation.data_ptr() if rotation is not None else None,
-        *(q.stride()[:2] if q is not None else (0, 0)), *k.stride()[:2],
-        *v.stride()[:2], *(q_out.stride()[:2] if q is not None else (0, 0)),
-        rotation.stride(0) if rotation is not None else 0,
-        rotary, int(interleaved), int(fill))
-    _launch(k, _lib().kv_append, kv, args)
+    q_at = out_at = at = rotary = 0
+    q_step = out_step = (0, 0)
+    if q is not None:
+        q_at, q_step = _place("q", q)
+        out_at, out_step = _place("q_out", q_out)
+    k_at, k_step = _place("k", k)
+    v_at, v_step = _place("v", v)
+    row = 0
+    if rotation is not None:
+        at, rotary = rotation.data_ptr(), rotation.shape[1]
+        row, last = rotation.stride()
+        if last != 1 or row % 4 or at % 16:
+            raise ValueError("rotation: rows are not contiguous at 16 bytes")
+    args = hiputil.KV_APPEND.pack(
+        q_at, k_at, v_at, out_at, at, *q_step, *k_step, *v_step, *out_step,
+        row, rotary, interleaved, fill)
+    kv = _pack(cache, k, heads, table, lens, starts, batch, per_seq)
+    device = k.get_device()
+    with _on(device):
+        _lib().kv_append(kv, args, _stream(device))
     return q_out
 
 
@@ -190,7 +182,7 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor,
     Rows of no sequence give the same in a new tensor and are left as they
     are in `out` (their logarithm is -inf in both)."""
     total, heads, dim = _rows("q", q)
-    kv = _describe(cache, q, heads, table, lens, starts)
+    batch, per_seq = _check(cache, q, heads, table, lens, starts)
     if dim not in ATTEND_DIMS:
         raise ValueError(f"dim {dim} is not one of {ATTEND_DIMS}")
     if scale is None:
@@ -201,165 +193,202 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor,
         window = 0
     elif window < 1:
         raise ValueError(f"window {window} is less than 1")
-    window = min(window, 2**31 - 1)
-    if starts is None:
-        max_new = total // kv.batch if kv.batch else 0
-    elif max_new is None:
+    if max_new is None:
         max_new = total
     elif max_new < 0:
         raise ValueError(f"max_new {max_new} is negative")
     fill = out is None
     if fill:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     else:
-        _like("out", out, q, heads=True)
-        if out.shape != q.shape:
-            raise ValueError("out is not shaped as q")
+        _like("out", out, q)
     _forward_only(q, out)
-    lse = None
+    result, lse, lse_at = out, None, 0
     if return_lse:
-        lse = torch.empty((total, heads), dtype=torch.float32,
-                          device=q.device)
-    result = (out, lse) if return_lse else out
+        lse = q.new_empty((total, heads), dtype=torch.float32)
+        result, lse_at = (out, lse), lse.data_ptr()
     if total == 0:
         return result
     if not q.is_cuda:
         _attend_plain(cache, q, table, lens, starts, scale, window, out, lse,
                       fill)
         return result
-    _strides("q", q, 8)
-    _strides("out", out, 8)
-    args = hiputil.KvAttend(
-        q.data_ptr(), out.data_ptr(),
-        lse.data_ptr() if lse is not None else None, *q.stride()[:2],
-        *out.stride()[:2], scale, window, min(max_new, total), int(fill), None)
-    size = _lib().kv_attend_work(kv, args)
-    if size:
-        work = torch.empty(size, dtype=torch.uint8, device=q.device)
-        args.work = work.data_ptr()
-    _launch(q, _lib().kv_attend, kv, args)
+    q_at, q_step = _place("q", q)
+    out_at, out_step = _place("out", out)
+    args = hiputil.KV_ATTEND.pack(
+        q_at, out_at, lse_at, *q_step, *out_step, scale,
+        min(window, 2**31 - 1), min(max_new, total), fill)
+    kv = _pack(cache, q, heads, table, lens, starts, batch, per_seq)
+    device = q.get_device()
+    lib = _lib()
+    size = lib.kv_attend_work(kv, args)
+    work = q.new_empty(size, dtype=torch.uint8) if size else None
+    with _on(device):
+        lib.kv_attend(kv, args, work.data_ptr() if size else None,
+                      _stream(device))
     return result
 
 
 # -- arguments ---------------------------------------------------------
+#
+# A step of a few tokens takes the GPU less time than it takes Python to
+# look its arguments over with care, so each check is one condition, and
+# what exactly is wrong is found out once it has failed.
 
 
-def _rows(name: str, t: torch.Tensor) -> tuple[int, int, int]:
-    if t.dim() != 3:
+def _rows(name: str, t: torch.Tensor) -> torch.Size:
+    shape = t.shape
+    if len(shape) != 3:
         raise ValueError(f"{name}: [total, heads, dim] is wanted, got "
-                         f"{tuple(t.shape)}")
-    if t.dtype not in (torch.bfloat16, torch.float16):
+                         f"{tuple(shape)}")
+    if t.dtype not in _ROW_TYPES:
         raise ValueError(f"{name}: bfloat16 or float16 is wanted, got "
                          f"{t.dtype}")
-    if t.shape[0] * t.shape[1] >= 2**31 - 1:
-        raise ValueError(f"{name}: {t.shape[0]} rows of {t.shape[1]} heads "
-                         "pass 31 bits")
-    return t.shape
+    if shape[0] * shape[1] >= 2**31 - 1:
+        raise ValueError(f"{name}: {shape[0]} rows of {shape[1]} heads pass "
+                         "31 bits")
+    return shape
 
 
 def _like(name: str, t: torch.Tensor, k: torch.Tensor,
           heads: bool = False) -> None:
     """`t` has the rows, type and device of `k`, and its heads or others."""
-    if (t.dim() != 3 or t.dtype != k.dtype
-            or t.get_device() != k.get_device() or t.shape[0] != k.shape[0]
-            or t.shape[2] != k.shape[2]
-            or (not heads and t.shape[1] != k.shape[1])):
+    a, b = t.shape, k.shape
+    if (t.dtype != k.dtype or t.get_device() != k.get_device()
+            or (a != b and not (heads and len(a) == 3 and a[0] == b[0]
+                                and a[2] == b[2]))):
         raise ValueError(
-            f"{name}: {t.dtype} {tuple(t.shape)} on {t.device} does not go "
-            f"with {k.dtype} {tuple(k.shape)} on {k.device}")
+            f"{name}: {t.dtype} {tuple(a)} on {t.device} does not go with "
+            f"{k.dtype} {tuple(b)} on {k.device}")
 
 
-def _strides(name: str, t: torch.Tensor, step: int) -> None:
-    """Each head's values are contiguous and begin at 16 bytes."""
-    *outer, last = t.stride()
-    if last != 1 or any(s % step for s in outer) or t.data_ptr() % 16:
-        raise ValueError(f"{name}: values of a head are not contiguous at "
-                         f"16 bytes (strides {t.stride()})")
+def _place(name: str, t: torch.Tensor) -> tuple[int, tuple[int, int]]:
+    """Address and strides of rows [total, heads, dim]."""
+    at = t.data_ptr()
+    row, head, last = t.stride()
+    if last != 1 or (row | head) % 8 or at % 16:
+        raise ValueError(_unaligned(name, t))
+    return at, (row, head)
 
 
-def _index(name: str, t: torch.Tensor, shape: tuple, device: int) -> None:
-    if (t.dtype != torch.int32 or t.shape != shape
-            or t.get_device() != device or (shape[0] > 1
-                                            and t.stride(0) != 1)):
-        raise ValueError(
-            f"{name}: a contiguous int32 {list(shape)} tensor on the rows' "
-            f"device is wanted, got {t.dtype} {tuple(t.shape)} on "
-            f"{t.device}")
+def _unaligned(name: str, t: torch.Tensor) -> str:
+    return (f"{name}: values of a head are not contiguous at 16 bytes "
+            f"(strides {t.stride()})")
 
 
-def _describe(cache: PagedCache, rows: torch.Tensor, heads: int,
-              table: torch.Tensor, lens: torch.Tensor,
-              starts: torch.Tensor | None) -> hiputil.KvCache:
-    """The checked arguments that both operators share."""
+def _check(cache: PagedCache, rows: torch.Tensor, heads: int,
+           table: torch.Tensor, lens: torch.Tensor,
+           starts: torch.Tensor | None) -> tuple[int, int]:
+    """What both operators ask of their common arguments; the table's
+    shape."""
     ck, cv, k_scale, v_scale = cache
-    device = rows.get_device()
-    total, _, dim = rows.shape
-    if ck.dim() != 4 or ck.shape != cv.shape or ck.dtype != cv.dtype:
+    device, total = rows.get_device(), rows.shape[0]
+    shape, dtype = ck.shape, ck.dtype
+    if (len(shape) != 4 or shape != cv.shape or dtype != cv.dtype
+            or shape[3] != rows.shape[2] or ck.get_device() != device
+            or cv.get_device() != device):
         raise ValueError(
-            f"cache: keys {ck.dtype} {tuple(ck.shape)} and values "
-            f"{cv.dtype} {tuple(cv.shape)} are not alike "
-            "[pages, page_size, kv_heads, dim]")
-    pages, page_size, kv_heads, cache_dim = ck.shape
-    if cache_dim != dim or ck.get_device() != device \
-            or cv.get_device() != device:
-        raise ValueError(f"cache: dim {cache_dim} on {ck.device} does not "
-                         f"go with rows of dim {dim} on {rows.device}")
-    if pages == 0 or page_size == 0 or kv_heads == 0 or heads % kv_heads \
-            or heads == 0:
+            f"cache: keys {dtype} {tuple(shape)} on {ck.device} and values "
+            f"{cv.dtype} {tuple(cv.shape)} on {cv.device} are not both "
+            f"[pages, page_size, kv_heads, {rows.shape[2]}] on "
+            f"{rows.device}")
+    pages, page_size, kv_heads, _ = shape
+    if (heads == 0 or kv_heads == 0 or heads % kv_heads or pages == 0
+            or page_size == 0 or max(pages, page_size) > 2**31 - 1):
         raise ValueError(f"cache: {pages} pages of {page_size} with "
                          f"{kv_heads} heads cannot serve {heads} heads")
-    if pages > 2**31 - 1 or page_size > 2**31 - 1:
-        raise ValueError("cache: pages or page_size pass 31 bits")
-    e4m3 = ck.dtype == torch.float8_e4m3fn
-    if not e4m3 and ck.dtype != rows.dtype:
-        raise ValueError(f"cache: {ck.dtype} is neither {rows.dtype} nor "
+    if dtype == torch.float8_e4m3fn:
+        for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if (s is None or s.dtype != torch.float32
+                    or s.shape != (kv_heads,) or s.get_device() != device
+                    or not s.is_contiguous()):
+                raise ValueError(
+                    f"{name}: float8_e4m3fn wants a contiguous float32 "
+                    f"[{kv_heads}] tensor on the cache's device")
+    elif dtype != rows.dtype:
+        raise ValueError(f"cache: {dtype} is neither {rows.dtype} nor "
                          "float8_e4m3fn")
-    for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if (s is not None) != e4m3:
-            raise ValueError(f"{name}: wanted with float8_e4m3fn, and only "
-                             "there")
-        if e4m3 and (s.dtype != torch.float32 or s.shape != (kv_heads,)
-                     or s.get_device() != device or not s.is_contiguous()):
-            raise ValueError(f"{name}: a contiguous float32 [{kv_heads}] "
-                             "tensor on the cache's device is wanted")
-    if ck.is_cuda:
-        _strides("cache.k", ck, 16 if e4m3 else 8)
-        _strides("cache.v", cv, 16 if e4m3 else 8)
-    if table.dim() != 2 or table.dtype != torch.int32 \
-            or table.get_device() != device \
-            or (table.shape[1] > 1 and table.stride(1) != 1):
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError(f"{'k' if k_scale is not None else 'v'}_scale: "
+                         f"{dtype} goes without")
+    if (table.dtype != torch.int32 or table.dim() != 2
+            or table.get_device() != device
+            or (table.shape[1] > 1 and table.stride(1) != 1)):
         raise ValueError(
-            f"table: an int32 [batch, pages] tensor with contiguous rows on "
+            "table: an int32 [batch, pages] tensor with contiguous rows on "
             f"the rows' device is wanted, got {table.dtype} "
             f"{tuple(table.shape)} on {table.device}")
     batch, per_seq = table.shape
     if per_seq * page_size > 2**31 - 1:
         raise ValueError(f"table: {per_seq} pages of {page_size} pass 31 "
                          "bits of positions")
-    _index("lens", lens, (batch,), device)
+    if (lens.dtype != torch.int32 or lens.shape != (batch,)
+            or lens.get_device() != device or not lens.is_contiguous()):
+        raise ValueError(_no_index("lens", lens, batch))
     if starts is not None:
-        _index("starts", starts, (batch + 1,), device)
-    elif (total % batch if batch else total):
+        if (starts.dtype != torch.int32 or starts.shape != (batch + 1,)
+                or starts.get_device() != device
+                or not starts.is_contiguous()):
+            raise ValueError(_no_index("starts", starts, batch + 1))
+    elif total % batch if batch else total:
         raise ValueError(f"{total} rows are not the same number for each of "
                          f"{batch} sequences: give starts")
     if total and (batch == 0 or per_seq == 0):
         raise ValueError("table: rows, but no sequences or no pages")
-    return hiputil.KvCache(
-        ck.data_ptr(), cv.data_ptr(),
-        k_scale.data_ptr() if e4m3 else None,
-        v_scale.data_ptr() if e4m3 else None,
-        table.data_ptr(), lens.data_ptr(),
-        starts.data_ptr() if starts is not None else None,
-        table.stride(0), *ck.stride()[:3], *cv.stride()[:3],
-        _TYPES[rows.dtype], _TYPES[ck.dtype], batch, total, heads, kv_heads,
-        dim, pages, page_size, per_seq)
+    return batch, per_seq
+
+
+def _no_index(name: str, t: torch.Tensor, n: int) -> str:
+    return (f"{name}: a contiguous int32 [{n}] tensor on the rows' device "
+            f"is wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _check_rotation(rotation: torch.Tensor, k: torch.Tensor,
+                    positions: int) -> None:
+    if (rotation.dim() != 2 or rotation.dtype != torch.float32
+            or rotation.get_device() != k.get_device()):
+        raise ValueError("rotation: a float32 [positions, rotary] tensor on "
+                         "the device of k is wanted")
+    have, rotary = rotation.shape
+    if rotary == 0 or rotary % 16 or rotary > k.shape[2]:
+        raise ValueError(f"rotation: {rotary} dimensions are no multiple of "
+                         f"16 up to {k.shape[2]}")
+    if have < positions:
+        raise ValueError(f"rotation: {have} positions, the table names "
+                         f"{positions}")
+
+
+def _pack(cache: PagedCache, rows: torch.Tensor, heads: int,
+          table: torch.Tensor, lens: torch.Tensor,
+          starts: torch.Tensor | None, batch: int, per_seq: int) -> bytes:
+    ck, cv, k_scale, v_scale = cache
+    pages, page_size, kv_heads, dim = ck.shape
+    *k_step, k_last = ck.stride()
+    *v_step, v_last = cv.stride()
+    k_at, v_at = ck.data_ptr(), cv.data_ptr()
+    step = 8 if k_scale is None else 16
+    if k_last != 1 or (k_step[0] | k_step[1] | k_step[2]) % step \
+            or k_at % 16:
+        raise ValueError(_unaligned("cache.k", ck))
+    if v_last != 1 or (v_step[0] | v_step[1] | v_step[2]) % step \
+            or v_at % 16:
+        raise ValueError(_unaligned("cache.v", cv))
+    return hiputil.KV_CACHE.pack(
+        k_at, v_at, 0 if k_scale is None else k_scale.data_ptr(),
+        0 if v_scale is None else v_scale.data_ptr(), table.data_ptr(),
+        lens.data_ptr(), 0 if starts is None else starts.data_ptr(),
+        table.stride(0), *k_step, *v_step, _TYPES[rows.dtype],
+        _TYPES[ck.dtype], batch, rows.shape[0], heads, kv_heads, dim, pages,
+        page_size, per_seq)
 
 
 def _forward_only(*tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in tensors):
-        raise ValueError("forward only: call under torch.no_grad(), or "
-                         "detach the arguments")
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError("forward only: call under torch.no_grad(), or "
+                             "detach the arguments")
 
 
 @functools.cache
@@ -367,13 +396,26 @@ def _lib() -> hiputil.HipUtil:
     return hiputil.load()
 
 
-def _launch(rows: torch.Tensor, entry, kv, args) -> None:
-    device = rows.get_device()
-    if device == torch.cuda.current_device():
-        entry(kv, args, torch.cuda.current_stream().cuda_stream)
-        return
-    with torch.cuda.device(device):
-        entry(kv, args, torch.cuda.current_stream().cuda_stream)
+# torch.cuda.current_stream() takes as long as the rest of a launch.
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+class _on:
+    """The device made current, where it is not."""
+
+    __slots__ = ("device", "before")
+
+    def __init__(self, device: int) -> None:
+        self.device = device
+
+    def __enter__(self) -> None:
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.device:
+            torch.cuda.set_device(self.device)
+
+    def __exit__(self, *exc) -> None:
+        if self.before != self.device:
+            torch.cuda.set_device(self.before)
 
 
 # -- plain forms, for tensors on the CPU -------------------------------

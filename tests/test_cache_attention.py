@@ -890,14 +890,17 @@ def test_entry_refuses_what_the_kernels_cannot_take():
     if not artifacts().hiputil.exists():
         pytest.skip("libnvshare_hiputil.so is not built")
     lib = hiputil.load()
-    kv, app, att = hiputil.KvCache(), hiputil.KvAppend(), hiputil.KvAttend()
-    for call, args in ((lib.kv_append, app), (lib.kv_attend, att)):
+    kv, app, att = (bytes(x.size) for x in (
+        hiputil.KV_CACHE, hiputil.KV_APPEND, hiputil.KV_ATTEND))
+    for call in (lambda: lib.kv_append(kv, app, 0),
+                 lambda: lib.kv_attend(kv, att, 0, 0),
+                 lambda: lib.kv_attend_work(kv, att)):
         with pytest.raises(RuntimeError, match="hipError_t=1"):
-            call(kv, args, 0)
+            call()
 
 
 def test_structures_match_the_header():
-    """hiputil's structures name the header's fields in its order."""
+    """hiputil's structures have the header's members in its order."""
     import re
 
     from nvshare_amd import hiputil
@@ -905,21 +908,18 @@ def test_structures_match_the_header():
 
     text = (REPO_ROOT / "hip" / "kvcache.h").read_text()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
-    kinds = {"int64_t": hiputil.ctypes.c_int64, "int": hiputil.ctypes.c_int,
-             "float": hiputil.ctypes.c_float}  # and pointers
-    for struct, cls in (("nvs_kv", hiputil.KvCache),
-                        ("nvs_kv_append_args", hiputil.KvAppend),
-                        ("nvs_kv_attend_args", hiputil.KvAttend)):
+    codes = {"int64_t": "q", "int": "i", "float": "f"}
+    for struct, packed in (("nvs_kv", hiputil.KV_CACHE),
+                           ("nvs_kv_append_args", hiputil.KV_APPEND),
+                           ("nvs_kv_attend_args", hiputil.KV_ATTEND)):
         body = re.search(r"struct %s \{(.*?)\};" % struct, text, re.S)[1]
-        want = []
+        names, code = [], ""
         for line in body.split(";"):
             m = re.match(r"\s*(?:const )?(\w+) (.*)", line, re.S)
             if m:
                 for name in m[2].split(","):
                     name = name.strip()
-                    kind = (hiputil.ctypes.c_void_p if name.startswith("*")
-                            else kinds[m[1]])
-                    want.append((name.lstrip("*"), kind))
-        assert cls._fields_ == want
-
-
+                    code += "P" if name.startswith("*") else codes[m[1]]
+                    names.append(name.lstrip("*"))
+        assert packed.names == names
+        assert packed.format == "@" + code + "0P"
