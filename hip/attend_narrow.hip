@@ -58,6 +58,7 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 	typedef narrow<T, C, D, NC, W> N;
 	constexpr int TILE = N::TILE, RB = N::RB, NI = N::NI;
 	__shared__ __attribute__((aligned(16))) char lds[N::LDS];
+	__shared__ int entries[W][2][64];
 	__shared__ float tops[W][16 * NC], sums[W][16 * NC];
 	const int lane = threadIdx.x & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -79,6 +80,8 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 
 	char *const k_lds = lds + wave * 2 * TILE * RB;
 	char *const v_lds = k_lds + TILE * RB;
+	const unsigned k_at = lds_at(lds) + wave * 2 * TILE * RB;
+	const unsigned v_at = k_at + TILE * RB;
 	const int *const table = c.table + (int64_t)b * c.table_row;
 	const float vs = sizeof(C) == 1 ? c.v_scale[kh] : 1.f;
 	const factor f = factor_of(a.scale * 1.44269504f *
@@ -125,6 +128,7 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 								   32 * d +
 								   8 * quarter);
 					q[n][d] = (q[n][d] ^ f.flip) & f.keep;
+					arrived(q[n][d]);
 				}
 			} else {
 #pragma unroll
@@ -134,11 +138,12 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 		}
 		/* The limits of all rows: keys up to `all` are seen by each
 		 * unless a window ends before. */
-		const int all = (int)min(max(s.pos + i0, (int64_t)-1),
-					 (int64_t)k.hi - 1);
+		const int all = uniform((int)min(max(s.pos + i0, (int64_t)-1),
+						 (int64_t)k.hi - 1));
 		const int any_low =
-			a.window > 0 ? (int)max(s.pos + i1 - a.window + 1,
-						(int64_t)0) :
+			a.window > 0 ? uniform((int)max(s.pos + i1 -
+								a.window + 1,
+							(int64_t)0)) :
 				       0;
 		const bool alike = s.pos + i0 == s.pos + i1;
 
@@ -151,43 +156,44 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 				out[n][d] = f32x4{};
 
 		/* Request a tile's rows.  `pages` has the page of key lane %
-		 * 32 of the tile; whole: all are in the same.  The addresses
+		 * 32 of the tile; whole: all are in the same.  Addresses
 		 * are made anew each time: kept ones would take more
 		 * registers than the results. */
+		constexpr int SIZE = sizeof(C);
 		auto request = [&](const void *cache, int64_t page_stride,
 				   int64_t slot_stride, int64_t head, int tile,
 				   int pages, bool whole, bool values,
-				   char *to) {
-			constexpr int SIZE = sizeof(C);
+				   unsigned to) {
 			const int key = tile * TILE;
+			const char *from = (const char *)cache +
+					   kh * head * SIZE;
 			int r = lr;
 
 			if (whole) {
 				const int page =
 					__builtin_amdgcn_readfirstlane(pages);
-				const char *from =
-					(const char *)cache +
-					(page * page_stride +
-					 slot_of(c, p, key) * slot_stride +
-					 kh * head) * SIZE;
+				const unsigned step =
+					(unsigned)(slot_stride * SIZE);
+
+				from += (page * page_stride +
+					 slot_of(c, p, key) * slot_stride) *
+					SIZE;
 #pragma unroll
 				for (int i = 0; i < NI; i++) {
 					asm volatile("" : "+v"(r));
 					const int row = i * N::RI + r;
-					const int piece =
+					const unsigned piece =
 						lc ^ (values ? N::turn_v(row) :
 							       N::turn_k(row));
 
-					copy_to_lds(from +
-							    row * slot_stride *
-								    SIZE +
-							    piece * 16,
+					copy_to_lds(from + (row * step +
+							    piece * 16),
 						    to + i * 1024);
 				}
 				return;
 			}
-			const char *base = (const char *)cache +
-					   kh * head * SIZE;
+			const int slots =
+				slot_of(c, p, key + (lane & (TILE - 1)));
 #pragma unroll
 			for (int i = 0; i < NI; i++) {
 				asm volatile("" : "+v"(r));
@@ -196,47 +202,63 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 								N::turn_v(row) :
 								N::turn_k(row));
 				const int page = __shfl(pages, row);
-				const char *from =
-					base + (page * page_stride +
-						slot_of(c, p, key + row) *
-							slot_stride) *
+				const int slot = __shfl(slots, row);
+				const char *at =
+					from + (page * page_stride +
+						slot * slot_stride) *
 						       SIZE;
 
 				if (page < 0)
-					from = (const char *)no_value;
-				copy_to_lds(from + piece * 16, to + i * 1024);
+					at = (const char *)no_value;
+				copy_to_lds(at + piece * 16, to + i * 1024);
 			}
 		};
-		auto is_whole = [&](int pages, int tile) {
-			return __all(pages >= 0) &&
-			       (c.page_size % TILE == 0);
+		const bool one_page = c.page_size % TILE == 0 && p.near_slots;
+		auto is_whole = [&](int pages) {
+			return one_page && __all(pages >= 0);
 		};
-		auto lookup = [&](int tile) {
-			if (tile >= last)
-				return -1;
-			return page_of(c, p, table,
-				       tile * TILE + (lane & (TILE - 1)), k);
+		/* The table's entry for key lane % 32 of a tile, or the
+		 * nearest one that some row sees. */
+		auto entry = [&](int tile) {
+			const int key = tile * TILE + (lane & (TILE - 1));
+
+			return table + entry_of(p, min(max(key, k.lo),
+						       k.hi - 1));
+		};
+		/* The pages, -1 for keys that no row sees. */
+		auto pages_of = [&](int tile, int entry) {
+			const int key = tile * TILE + (lane & (TILE - 1));
+
+			return key >= k.lo && key < k.hi && is_page(c, entry) ?
+				       entry :
+				       -1;
 		};
 
-		int t = first + wave;
-		int pages = lookup(t), next = lookup(t + W);
-		bool whole = is_whole(pages, t);
+		/* On their way at the loop's head, in this order: the table's
+		 * entries for the next tile, this one's keys, its values. */
+		int t = first + wave, turn = 0;
+		int pages = -1;
+		bool whole = false;
 
 		if (t < last) {
+			pages = pages_of(t, *entry(t));
+			whole = is_whole(pages);
+			copy4_to_lds(entry(t + W), lds_at(entries[wave][0]));
 			request(c.k_cache, c.k_page, c.k_slot, c.k_head, t,
-				pages, whole, false, k_lds);
+				pages, whole, false, k_at);
 			request(c.v_cache, c.v_page, c.v_slot, c.v_head, t,
-				pages, whole, true, v_lds);
+				pages, whole, true, v_at);
 		}
-		for (; t < last; t += W) {
-			const unsigned valid =
-				(unsigned)__ballot(pages >= 0);
-			const int pages1 = next;
-			const bool whole1 = is_whole(pages1, t + W);
+		for (; t < last; t += W, turn ^= 1) {
+			const unsigned valid = (unsigned)__ballot(pages >= 0);
 			const bool more = t + W < last;
 			const int key0 = t * TILE;
 
-			next = lookup(t + 2 * W);
+			wait_loads<NI>();
+			const int pages1 =
+				pages_of(t + W, entries[wave][turn][lane]);
+			const bool whole1 = is_whole(pages1);
+
 			/* Keys: S^T = K Q^T. */
 			wait_loads<NI>();
 			f32x4 score[NC][2];
@@ -282,10 +304,13 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 				}
 			}
 			wait_lds();
-			if (more)
+			if (more) {
+				copy4_to_lds(entry(t + 2 * W),
+					     lds_at(entries[wave][turn ^ 1]));
 				request(c.k_cache, c.k_page, c.k_slot,
 					c.k_head, t + W, pages1, whole1, false,
-					k_lds);
+					k_at);
+			}
 
 			/* Weights. */
 			const bool masked = valid != ~0u ||
@@ -302,16 +327,23 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 					for (int j = 0; j < 4; j++)
 						x[4 * h + j] = score[n][h][j];
 				if (masked) {
+					rarely();
+					/* As seen from the first key. */
+					const unsigned mine =
+						valid >> 4 * quarter;
+					const int to = lim[n] - key0 -
+						       4 * quarter;
+					const int after = low[n] - key0 -
+							  4 * quarter;
 #pragma unroll
 					for (int e = 0; e < 8; e++) {
-						const int j =
-							16 * (e >> 2) +
-							4 * quarter + (e & 3);
+						const int j = 16 * (e >> 2) +
+							      (e & 3);
+						const bool sees =
+							(mine >> j & 1) &
+							(j <= to) & (j > after);
 
-						if (!(valid >> j & 1) ||
-						    key0 + j > lim[n] ||
-						    key0 + j <= low[n])
-							x[e] = -INFINITY;
+						x[e] = sees ? x[e] : -INFINITY;
 					}
 				}
 				float most = x[0];
@@ -344,7 +376,7 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 
 			/* Values: O^T += V^T P^T. */
 			if (more)
-				wait_loads<NI>();
+				wait_loads<NI + 1>();
 			else
 				wait_loads<0>();
 			auto value = [&](int d) {
@@ -413,6 +445,7 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 			bool odd = false;
 
 			if (masked && !alike)
+#pragma unroll 2
 				for (int i = 0; i < NI; i++) {
 					const u32x4 w =
 						*(const u32x4 *)(v_lds +
@@ -478,7 +511,7 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 			if (more)
 				request(c.v_cache, c.v_page, c.v_slot,
 					c.v_head, t + W, pages1, whole1, true,
-					v_lds);
+					v_at);
 			pages = pages1;
 			whole = whole1;
 		}

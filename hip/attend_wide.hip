@@ -116,21 +116,16 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 	const int w0 = min(rows - 1, r0 + wave * 32) / group;
 	const int w1 = min(rows - 1, r0 + wave * 32 + 31) / group;
 	const bool idle = r0 + wave * 32 >= rows;
-	const int all = limit(w0), most_lim = limit(w1);
-	const int any_low = a.window > 0 ?
-				    (int)max(s.pos + w1 - a.window + 1,
-					     (int64_t)0) :
-				    0;
-	const int least_low = a.window > 0 ?
-				      (int)max(s.pos + w0 - a.window + 1,
-					       (int64_t)0) :
+	const int all = uniform(limit(w0)), most_lim = uniform(limit(w1));
+	auto lowest = [&](int i) {
+		return a.window > 0 ? uniform((int)max(
+					      s.pos + i - a.window + 1,
+					      (int64_t)0)) :
 				      0;
+	};
+	const int any_low = lowest(w1), least_low = lowest(w0);
 	/* Where the block's rows do not all see the same. */
-	const int block_all = limit(i0);
-	const int block_low = a.window > 0 ?
-				      (int)max(s.pos + i1 - a.window + 1,
-					       (int64_t)0) :
-				      0;
+	const int block_all = uniform(limit(i0)), block_low = lowest(i1);
 	const bool alike = i0 == i1;
 
 	u32x4 q[D / 16];
@@ -142,6 +137,7 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 		if (real)
 			q[d] = *(const u32x4 *)(src + 16 * d + 8 * half);
 		q[d] = (q[d] ^ f.flip) & f.keep;
+		arrived(q[d]);
 	}
 
 	softmax<T> sm;
@@ -152,81 +148,118 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 		for (int e = 0; e < 16; e++)
 			out[d][e] = 0.f;
 
-	/* The pages of a tile's keys, key lane of it in lane `lane`. */
+	/* The page of key `lane` of a tile. */
 	auto lookup = [&](int tile) {
-		if (tile >= last)
-			return -1;
-		return page_of(c, p, table, tile * TILE + lane, k);
+		return tile < last ? look_up(p, table, tile * TILE + lane, k) :
+				     -1;
 	};
+	/* Whether a tile lies in one page as a whole. */
+	const bool one_page = c.page_size % TILE == 0 && p.near_slots;
 	auto is_whole = [&](int pages) {
-		return __all(pages >= 0) && c.page_size % TILE == 0;
+		return one_page && __all(is_page(c, pages));
 	};
 	constexpr int SIZE = sizeof(C);
-	/* Where a tile's row begins in the cache. */
-	auto row_of = [&](const void *cache, int64_t page_stride,
-			  int64_t slot_stride, int64_t head_stride, int key,
-			  int pages, bool whole, int row) {
-		const char *base = (const char *)cache + kh * head_stride * SIZE;
+	const char *const k_head = (const char *)c.k_cache +
+				   kh * c.k_head * SIZE;
+	const char *const v_head = (const char *)c.v_cache +
+				   kh * c.v_head * SIZE;
+	const unsigned k_step = (unsigned)(c.k_slot * SIZE);
+	const unsigned v_step = (unsigned)(c.v_slot * SIZE);
+	/* Where a tile that lies in one page begins. */
+	auto tile_at = [&](const char *head, int64_t page_stride,
+			   int64_t slot_stride, int key, int pages) {
+		const int page = __builtin_amdgcn_readfirstlane(pages);
 
-		if (whole) {
-			const int page = __builtin_amdgcn_readfirstlane(pages);
-
-			return base +
-			       (page * page_stride +
-				slot_of(c, p, key) * slot_stride) *
-				       SIZE +
-			       row * slot_stride * SIZE;
-		}
-		const int page = __shfl(pages, row);
-
-		if (page < 0)
-			return (const char *)no_value;
-		return base + (page * page_stride +
-			       slot_of(c, p, key + row) * slot_stride) *
+		return head + (page * page_stride +
+			       slot_of(c, p, key) * slot_stride) *
 				      SIZE;
 	};
+	/* Where a key's row begins; pages and slots are those of key `lane`
+	 * of the tile. */
+	auto row_at = [&](const char *head, int64_t page_stride,
+			  int64_t slot_stride, int pages, int slots, int row) {
+		const int page = __shfl(pages, row), slot = __shfl(slots, row);
+
+		return !is_page(c, page) ?
+			       (const char *)no_value :
+			       head + (page * page_stride +
+					  slot * slot_stride) *
+						 SIZE;
+	};
 	/* 16 bits: request a tile for buffer n. */
+	const int load_row = wave * NI * W::RI + lane / W::LR;
+	const int load_piece = lane % W::LR;
 	auto request = [&](int tile, int pages, int n) {
-		const bool whole = is_whole(pages);
 		const int key = tile * TILE;
-		char *to = lds + n * 2 * W::BUFFER + wave * NI * 1024;
-		const int lr = lane / W::LR, lc = lane % W::LR;
+		const unsigned to = lds_at(lds) + n * 2 * W::BUFFER +
+				    wave * NI * 1024;
+
+		if (is_whole(pages)) {
+			const char *k = tile_at(k_head, c.k_page, c.k_slot,
+						key, pages);
+			const char *v = tile_at(v_head, c.v_page, c.v_slot,
+						key, pages);
+#pragma unroll
+			for (int i = 0; i < NI; i++) {
+				const int row = load_row + i * W::RI;
+
+				copy_to_lds(k + (row * k_step +
+						 (load_piece ^ W::turn_k(row)) *
+							 16u),
+					    to + i * 1024);
+				copy_to_lds(v + (row * v_step +
+						 (load_piece ^ W::turn_v(row)) *
+							 16u),
+					    to + W::BUFFER + i * 1024);
+			}
+			return;
+		}
+		const int slots = slot_of(c, p, key + lane);
 #pragma unroll
 		for (int i = 0; i < NI; i++) {
-			const int row = (wave * NI + i) * W::RI + lr;
+			rarely();
+			const int row = load_row + i * W::RI;
 
-			copy_to_lds(row_of(c.k_cache, c.k_page, c.k_slot,
-					   c.k_head, key, pages, whole, row) +
-					    (lc ^ W::turn_k(row)) * 16,
+			copy_to_lds(row_at(k_head, c.k_page, c.k_slot, pages,
+					   slots, row) +
+					    (load_piece ^ W::turn_k(row)) * 16,
 				    to + i * 1024);
-			copy_to_lds(row_of(c.v_cache, c.v_page, c.v_slot,
-					   c.v_head, key, pages, whole, row) +
-					    (lc ^ W::turn_v(row)) * 16,
+			copy_to_lds(row_at(v_head, c.v_page, c.v_slot, pages,
+					   slots, row) +
+					    (load_piece ^ W::turn_v(row)) * 16,
 				    to + W::BUFFER + i * 1024);
 		}
 	};
 	/* e4m3: fetch a tile into registers, put it into buffer n. */
 	u32x4 hold[2][SIZE == 1 ? W::NP : 1];
 	auto fetch = [&](int tile, int pages) {
-		const bool whole = is_whole(pages);
 		const int key = tile * TILE;
+		const bool whole = is_whole(pages);
+		const int slots = slot_of(c, p, key + lane);
+		const char *k = nullptr, *v = nullptr;
+
+		if (whole) {
+			k = tile_at(k_head, c.k_page, c.k_slot, key, pages);
+			v = tile_at(v_head, c.v_page, c.v_slot, key, pages);
+		}
 #pragma unroll
 		for (int i = 0; i < W::NP; i++) {
 			const int n = i * 256 + threadIdx.x;
 			const int row = n / (D / 16), piece = n % (D / 16);
+			const char *from_k, *from_v;
 
-			hold[0][i] = *(const u32x4 *)(row_of(c.k_cache,
-							     c.k_page, c.k_slot,
-							     c.k_head, key,
-							     pages, whole,
-							     row) +
-						      piece * 16);
-			hold[1][i] = *(const u32x4 *)(row_of(c.v_cache,
-							     c.v_page, c.v_slot,
-							     c.v_head, key,
-							     pages, whole,
-							     row) +
-						      piece * 16);
+			if (whole) {
+				from_k = k + row * k_step;
+				from_v = v + row * v_step;
+			} else {
+				rarely();
+				from_k = row_at(k_head, c.k_page, c.k_slot,
+						pages, slots, row);
+				from_v = row_at(v_head, c.v_page, c.v_slot,
+						pages, slots, row);
+			}
+			hold[0][i] = *(const u32x4 *)(from_k + piece * 16);
+			hold[1][i] = *(const u32x4 *)(from_v + piece * 16);
 		}
 	};
 	auto put = [&](int n) {
@@ -267,7 +300,7 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 		const int n = (t - first) & 1;
 		const char *const k_lds = lds + n * 2 * W::BUFFER;
 		char *const v_lds = lds + n * 2 * W::BUFFER + W::BUFFER;
-		const uint64_t valid = __ballot(pages >= 0);
+		const uint64_t valid = __ballot(is_page(c, pages));
 		const int key0 = t * TILE;
 
 		/* This tile has come, and all are done with the other. */
@@ -380,20 +413,25 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 			/* Weights. */
 			if (valid != ~0ull || key0 + TILE - 1 > all ||
 			    key0 < any_low) {
+				rarely();
+				/* As seen from the lane's first key. */
+				const uint64_t mine = valid >> 4 * half;
+				const int to = lim - key0 - 4 * half;
+				const int after = low - key0 - 4 * half;
 #pragma unroll
 				for (int h = 0; h < 2; h++)
 #pragma unroll
 					for (int e = 0; e < 16; e++) {
-						const int j =
-							32 * h +
-							8 * (e >> 2) +
-							4 * half + (e & 3);
+						const int j = 32 * h +
+							      8 * (e >> 2) +
+							      (e & 3);
+						const bool sees =
+							(mine >> j & 1) &
+							(j <= to) & (j > after);
 
-						if (!(valid >> j & 1) ||
-						    key0 + j > lim ||
-						    key0 + j <= low)
-							score[h][e] =
-								-INFINITY;
+						score[h][e] = sees ?
+								      score[h][e] :
+								      -INFINITY;
 					}
 			}
 			float most = score[0][0];

@@ -41,7 +41,9 @@ struct nvs_plan {
 	int joined_rows; /* rows of a sequence that narrow parts may have */
 	int narrow_parts, wide_parts; /* blocks that may divide the keys */
 	int wide_blocks;	      /* blocks of rows, for one cached head */
-	int page_shift; /* log2 of page_size, -1 where it is no power of 2 */
+	uint64_t page_magic; /* key / page_size = key * magic >> shift */
+	int page_shift;
+	int near_slots; /* a tile's rows lie within 31 bits of each other */
 	int cover; /* the launch that sees to rows of no sequence: 1 narrow,
 		      2 wide */
 	/* Results and (log2 of the weights' unit, sum of the weights in it)
@@ -78,8 +80,8 @@ __device__ __forceinline__ key_range keys_of(const nvs_kv &c, int window,
 	const int64_t lo = window > 0 ? s.pos + i0 + 1 - window : 0;
 	key_range k;
 
-	k.lo = (int)min(max(lo, (int64_t)0), capacity);
-	k.hi = (int)max(hi, (int64_t)0);
+	k.lo = uniform((int)min(max(lo, (int64_t)0), capacity));
+	k.hi = uniform((int)max(hi, (int64_t)0));
 	if (k.hi <= k.lo) {
 		k.lo = k.hi = k.first = k.last = 0;
 		k.per = 1;
@@ -96,43 +98,82 @@ __device__ __forceinline__ int parts_of(const key_range &k)
 	return max(1, (k.last - k.first + k.per - 1) / k.per);
 }
 
-/* Page and slot of a position. */
-__device__ __forceinline__ int entry_of(const nvs_kv &c, const nvs_plan &p,
-					int key)
+/* The number in its sequence of the page of a position. */
+__device__ __forceinline__ int entry_of(const nvs_plan &p, int key)
 {
-	return p.page_shift >= 0 ? key >> p.page_shift : key / c.page_size;
+	return (int)((unsigned)key * p.page_magic >> p.page_shift);
 }
 
 __device__ __forceinline__ int slot_of(const nvs_kv &c, const nvs_plan &p,
 				       int key)
 {
-	return p.page_shift >= 0 ? key & (c.page_size - 1) :
-				   key % c.page_size;
+	return key - entry_of(p, key) * c.page_size;
 }
 
-/* The page of a key in [lo, hi); -1 for other keys and bad pages. */
-__device__ __forceinline__ int page_of(const nvs_kv &c, const nvs_plan &p,
-				       const int *table, int key,
-				       const key_range &k)
+/* The table's entry for a key in [lo, hi), -1 for other keys.  It is
+ * looked up a tile ahead and not looked at before that tile's turn, which
+ * would wait for it and for all loads before it. */
+__device__ __forceinline__ int look_up(const nvs_plan &p, const int *table,
+				       int key, const key_range &k)
 {
-	if (key < k.lo || key >= k.hi)
-		return -1;
-	const int page = table[entry_of(c, p, key)];
+	return key >= k.lo && key < k.hi ? table[entry_of(p, key)] : -1;
+}
 
-	return (unsigned)page < (unsigned)c.pages ? page : -1;
+/* Whether an entry is a page of the cache. */
+__device__ __forceinline__ bool is_page(const nvs_kv &c, int entry)
+{
+	return (unsigned)entry < (unsigned)c.pages;
 }
 
 /* Read in the place of keys and values that are none: a value that is not
  * seen still meets a weight of zero, so it has to be a finite number. */
 static __device__ const u32x4 no_value[32] = {};
 
-/* 16 bytes a lane from global memory to LDS, at `to` + 16 * lane; `to` is
- * the same for the whole wave. */
-__device__ __forceinline__ void copy_to_lds(const char *from, char *to)
+/* Where LDS memory lies, as the instructions count. */
+__device__ __forceinline__ unsigned lds_at(const void *p)
 {
-	__builtin_amdgcn_global_load_lds(
-		(const __attribute__((address_space(1))) void *)from,
-		(__attribute__((address_space(3))) void *)to, 16, 0, 0);
+	return (unsigned)(uintptr_t)(
+		const __attribute__((address_space(3))) char *)p;
+}
+
+/*
+ * 16 bytes (4) a lane from global memory to LDS, at `to` + 16 (4) * lane;
+ * `to` is the same for the whole wave.  In assembly, because for the
+ * builtin the compiler waits for all of a wave's loads before each read of
+ * LDS, and the tile that is on its way would have to come before the
+ * present one is read: the kernels wait by wait_loads() themselves.  There
+ * is no result in a register, and m0 has its one wait state before it is
+ * read.
+ */
+__device__ __forceinline__ void copy_to_lds(const char *from, unsigned to)
+{
+	asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\t"
+		     "global_load_lds_dwordx4 %0, off"
+		     :
+		     : "v"(from), "s"(uniform(to))
+		     : "memory", "m0");
+}
+
+__device__ __forceinline__ void copy4_to_lds(const int *from, unsigned to)
+{
+	asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\t"
+		     "global_load_lds_dword %0, off"
+		     :
+		     : "v"(from), "s"(uniform(to))
+		     : "memory", "m0");
+}
+
+/* Keeps the compiler from computing what is rarely wanted each time: a
+ * branch that has this is a branch. */
+__device__ __forceinline__ void rarely()
+{
+	asm volatile("");
+}
+
+/* Waits for a load here and not at each of its uses in a loop. */
+__device__ __forceinline__ void arrived(u32x4 &x)
+{
+	asm volatile("" : "+v"(x));
 }
 
 /* At most N of the wave's loads still under way; no LDS access moves

@@ -276,9 +276,18 @@ nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, void *work,
 
 	if (a.window > 0)
 		keys = keys < a.window + most_new ? keys : a.window + most_new;
-	p.page_shift = c.page_size & (c.page_size - 1) ?
-			       -1 :
-			       __builtin_ctz(c.page_size);
+	/* With 2^(l - 1) < page_size <= 2^l, ceil(2^(31 + l) / page_size)
+	 * divides numbers of 31 bits. */
+	int l = 0;
+
+	while (1ll << l < c.page_size)
+		l++;
+	p.page_shift = 31 + l;
+	p.page_magic = ((1ull << p.page_shift) + c.page_size - 1) /
+		       (uint64_t)c.page_size;
+	const int64_t slot = c.k_slot > c.v_slot ? c.k_slot : c.v_slot;
+
+	p.near_slots = slot < (1ll << 30) / WIDE_TILE;
 	p.span = most_rows > 32 || most_rows <= 16 ? 16 : 32;
 	p.narrow_rows = most_rows <= 32 ? 0x7fffffff : c.starts ? 16 : 0;
 	p.joined_rows = (int)(most_rows < p.span ? most_rows : p.span);

@@ -47,6 +47,13 @@ template <> struct types<fp16_t> {
 	static constexpr unsigned exponent = 0x7c007c00u, one = 0x04000400u;
 };
 
+/* A number that is the same in the whole wave, where the compiler does not
+ * see that it is. */
+__device__ __forceinline__ int uniform(int x)
+{
+	return __builtin_amdgcn_readfirstlane(x);
+}
+
 /* Two numbers rounded to nearest, ties to even. */
 template <typename T>
 __device__ __forceinline__ unsigned pack2(float a, float b)
