@@ -8,28 +8,32 @@ namespace {
 
 /*
  * A block has W waves and NC columns of 16 rows, all in every wave; wave w
- * takes each W-th tile of 32 keys.  A wave's tiles lie in LDS of its own,
- * filled by direct loads, so the waves never wait for each other: the next
- * tile's keys are requested as soon as this one's are read, its values as
- * soon as this one's are, and the loads of 4 to 16 waves a CU are under
- * way together.  What the waves have is added up in LDS at the end.
+ * takes each W-th tile of its block's keys.  A wave's tiles lie in LDS of
+ * its own, filled by direct loads, so the waves never wait for each other:
+ * the next tile's keys are requested as soon as this one's are read, its
+ * values as soon as this one's are, and the loads of 4 to 16 waves a CU
+ * are under way together.  What the waves have is added up in LDS at the
+ * end.
+ *
+ * A tile has 32 keys, 64 where 32 would be less than 8 KiB: what is done
+ * once a tile (its page, its mask, the maximum over the lanes) would take
+ * longer than its loads.
  */
 template <typename T, typename C, int D, int NC, int W> struct narrow {
-	static constexpr int TILE = NARROW_TILE;
-	static constexpr int RB = D * sizeof(C);  /* bytes of a row in LDS */
-	static constexpr int LR = RB / 16;	  /* lanes that load a row */
-	static constexpr int RI = 64 / LR;	  /* rows of a load */
-	static constexpr int NI = TILE / RI;	  /* loads of a tile */
+	static constexpr int RB = D * sizeof(C); /* bytes of a row in LDS */
+	static constexpr int TILE = nvs_narrow_tile(D, sizeof(C));
+	static constexpr int LR = RB / 16;  /* lanes that load a row */
+	static constexpr int RI = 64 / LR;  /* rows of a load */
+	static constexpr int NI = TILE / RI; /* loads of a tile */
 	static constexpr int STAGE = W * 2 * TILE * RB;
-	static constexpr int OUT_ROW = D + 4;	  /* floats, off the banks */
+	static constexpr int OUT_ROW = D + 4; /* floats, off the banks */
 	static constexpr int MERGE = W * 16 * NC * OUT_ROW * 4;
 	static constexpr int LDS = STAGE > MERGE ? STAGE : MERGE;
 	/* Waves that a SIMD holds: as LDS allows, and with 32 rows as the
 	 * registers do. */
-	static constexpr int WAVES = LDS > 80 * 1024 || W == 2 ? 1 :
-				     LDS * 4 <= 158 * 1024 && NC == 1 ?
-								 4 :
-								 2;
+	static constexpr int WAVES = LDS > 76 * 1024 || W == 2	   ? 1 :
+				     LDS <= 38 * 1024 && NC == 1 ? 4 :
+								     2;
 
 	/* Where a row's 16-byte pieces lie: turned about so that the 16
 	 * rows of a read fall on all banks. */
@@ -57,50 +61,99 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 {
 	typedef narrow<T, C, D, NC, W> N;
 	constexpr int TILE = N::TILE, RB = N::RB, NI = N::NI;
+	constexpr int SUBS = TILE / 32;
 	__shared__ __attribute__((aligned(16))) char lds[N::LDS];
 	__shared__ int entries[W][2][64];
 	__shared__ float tops[W][16 * NC], sums[W][16 * NC];
 	const int lane = threadIdx.x & 63;
-	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int wave = uniform(threadIdx.x >> 6);
 	const int col = lane & 15, quarter = lane >> 4;
-
-	const int kh = blockIdx.x % c.kv_heads;
-	const int part = blockIdx.x / c.kv_heads % p.narrow_parts;
-	const int b = blockIdx.x / c.kv_heads / p.narrow_parts;
 	const int group = c.heads / c.kv_heads;
-	const sequence s = sequence_of(c, b);
-	const int rows = s.count * group;
+
+	/* With 8 cached heads each has an XCD of its own.  (All heads of the
+	 * same keys on one XCD: 399 us where this takes 383, for 64 tokens
+	 * over 8192 keys each.) */
+	const int kh = blockIdx.x % c.kv_heads;
+	const int block = blockIdx.x / c.kv_heads;
 
 	if (p.cover == 1)
 		cover_padding<T>(c, a, blockIdx.x, gridDim.x);
-	if (rows > p.narrow_rows)
-		return;
-	/* A sequence with more rows than the caller said goes undivided. */
-	const int most_parts = rows > p.joined_rows ? 1 : p.narrow_parts;
 
 	char *const k_lds = lds + wave * 2 * TILE * RB;
 	char *const v_lds = k_lds + TILE * RB;
 	const unsigned k_at = lds_at(lds) + wave * 2 * TILE * RB;
 	const unsigned v_at = k_at + TILE * RB;
-	const int *const table = c.table + (int64_t)b * c.table_row;
 	const float vs = sizeof(C) == 1 ? c.v_scale[kh] : 1.f;
 	const factor f = factor_of(a.scale * 1.44269504f *
 				   (sizeof(C) == 1 ? c.k_scale[kh] : 1.f));
 	/* Which 16 bytes of a tile's rows this lane loads. */
 	const int lr = lane / N::LR, lc = lane % N::LR;
 
-	for (int r0 = 0; r0 < rows; r0 += 16 * NC) {
+	/* This block's share of all sequences' tiles, one after the other;
+	 * block 0 leaves where each begins for the join. */
+	const share mine = share_of(c, a, p, TILE, block,
+				    blockIdx.x == 0 && wave == 0);
+	int64_t at = mine.from; /* the next tile */
+	int b = mine.b, odd_b = block, odd_r0 = 0;
+	int64_t b_from = mine.b_from; /* the first tile of sequence b */
+
+	for (;;) {
+		/* The next piece: rows r0 and on of sequence b, its tiles
+		 * [first, last), and where its result goes. */
+		sequence s;
+		key_range k;
+		int r0 = 0, first, last, slot = -1;
+
+		if (at < mine.to && b < c.batch) {
+			s = sequence_of(c, b);
+			k = narrow_keys(c, a, p, s, TILE);
+			const int64_t b_to = b_from + narrow_tiles(c, p, s, k);
+
+			if (b_to <= at) {
+				b_from = b_to;
+				b++;
+				continue;
+			}
+			const int64_t to = min(b_to, mine.to);
+
+			first = k.first + (int)(at - b_from);
+			last = min(k.first + (int)(to - b_from), k.last);
+			if (at > b_from || to < b_to)
+				slot = at == mine.from ? 0 : 1;
+			at = to;
+		} else {
+			/* Sequences with more rows than the caller said:
+			 * undivided, so many rows at a time. */
+			if (!c.starts || p.narrow_rows < 0x7fffffff ||
+			    odd_b >= c.batch)
+				break;
+			b = odd_b;
+			s = sequence_of(c, b);
+			if (s.count * group <= p.joined_rows ||
+			    odd_r0 >= s.count * group) {
+				odd_b += p.narrow_blocks;
+				odd_r0 = 0;
+				continue;
+			}
+			r0 = odd_r0;
+			odd_r0 += 16 * NC;
+			k = keys_of(c, a.window, s, r0 / group,
+				    min(s.count,
+					(r0 + 16 * NC - 1) / group + 1) -
+					    1,
+				    TILE);
+			first = k.first;
+			last = k.last;
+		}
+		first = uniform(first);
+		last = uniform(last);
+		k.lo = uniform(k.lo);
+		k.hi = uniform(k.hi);
+		const int rows = s.count * group;
 		const int i0 = r0 / group;
 		const int i1 = min(s.count, (r0 + 16 * NC - 1) / group + 1) -
 			       1;
-		const key_range k = keys_of(c, a.window, s, i0, i1, TILE,
-					    NARROW_LEAST, most_parts);
-		const int parts = parts_of(k);
-
-		if (part >= parts)
-			continue;
-		const int first = k.first + part * k.per;
-		const int last = min(k.last, first + k.per);
+		const int *const table = c.table + (int64_t)b * c.table_row;
 
 		u32x4 q[NC][D / 32];
 		/* The lane's row sees keys in (low, lim]. */
@@ -128,7 +181,6 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 								   32 * d +
 								   8 * quarter);
 					q[n][d] = (q[n][d] ^ f.flip) & f.keep;
-					arrived(q[n][d]);
 				}
 			} else {
 #pragma unroll
@@ -147,6 +199,15 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 				       0;
 		const bool alike = s.pos + i0 == s.pos + i1;
 
+		/* Not before the first tile is on its way. */
+		auto queries_arrived = [&]() {
+#pragma unroll
+			for (int n = 0; n < NC; n++)
+#pragma unroll
+				for (int d = 0; d < D / 32; d++)
+					arrived(q[n][d]);
+		};
+
 		softmax<T> sm[NC];
 		f32x4 out[NC][D / 16];
 #pragma unroll
@@ -156,7 +217,7 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 				out[n][d] = f32x4{};
 
 		/* Request a tile's rows.  `pages` has the page of key lane %
-		 * 32 of the tile; whole: all are in the same.  Addresses
+		 * TILE of the tile; whole: all are in the same.  Addresses
 		 * are made anew each time: kept ones would take more
 		 * registers than the results. */
 		constexpr int SIZE = sizeof(C);
@@ -217,7 +278,7 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 		auto is_whole = [&](int pages) {
 			return one_page && __all(pages >= 0);
 		};
-		/* The table's entry for key lane % 32 of a tile, or the
+		/* The table's entry for key lane % TILE of a tile, or the
 		 * nearest one that some row sees. */
 		auto entry = [&](int tile) {
 			const int key = tile * TILE + (lane & (TILE - 1));
@@ -249,8 +310,9 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 			request(c.v_cache, c.v_page, c.v_slot, c.v_head, t,
 				pages, whole, true, v_at);
 		}
+		queries_arrived();
 		for (; t < last; t += W, turn ^= 1) {
-			const unsigned valid = (unsigned)__ballot(pages >= 0);
+			const uint64_t valid = __ballot(pages >= 0);
 			const bool more = t + W < last;
 			const int key0 = t * TILE;
 
@@ -261,9 +323,9 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 
 			/* Keys: S^T = K Q^T. */
 			wait_loads<NI>();
-			f32x4 score[NC][2];
+			f32x4 score[NC][2 * SUBS];
 #pragma unroll
-			for (int h = 0; h < 2; h++) {
+			for (int h = 0; h < 2 * SUBS; h++) {
 #pragma unroll
 				for (int n = 0; n < NC; n++)
 					score[n][h] = f32x4{};
@@ -313,34 +375,34 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 			}
 
 			/* Weights. */
-			const bool masked = valid != ~0u ||
+			const bool masked = valid != ~0ull ||
 					    key0 + TILE - 1 > all ||
 					    key0 < any_low;
-			u32x4 weight[NC];
+			u32x4 weight[NC][SUBS];
 #pragma unroll
 			for (int n = 0; n < NC; n++) {
-				float x[8];
+				float x[8 * SUBS];
 
 #pragma unroll
-				for (int h = 0; h < 2; h++)
+				for (int h = 0; h < 2 * SUBS; h++)
 #pragma unroll
 					for (int j = 0; j < 4; j++)
 						x[4 * h + j] = score[n][h][j];
 				if (masked) {
 					rarely();
 					/* As seen from the first key. */
-					const unsigned mine =
+					const uint64_t shown =
 						valid >> 4 * quarter;
 					const int to = lim[n] - key0 -
 						       4 * quarter;
 					const int after = low[n] - key0 -
 							  4 * quarter;
 #pragma unroll
-					for (int e = 0; e < 8; e++) {
+					for (int e = 0; e < 8 * SUBS; e++) {
 						const int j = 16 * (e >> 2) +
 							      (e & 3);
 						const bool sees =
-							(mine >> j & 1) &
+							(shown >> j & 1) &
 							(j <= to) & (j > after);
 
 						x[e] = sees ? x[e] : -INFINITY;
@@ -348,7 +410,7 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 				}
 				float most = x[0];
 #pragma unroll
-				for (int e = 1; e < 8; e++)
+				for (int e = 1; e < 8 * SUBS; e++)
 					most = fmaxf(most, x[e]);
 				f32x2 y = odd_even_quarters(most);
 				y = halves(fmaxf(y[0], y[1]));
@@ -362,16 +424,16 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 				}
 				const float unit = sm[n].unit(f.c);
 #pragma unroll
-				for (int e = 0; e < 8; e++) {
+				for (int e = 0; e < 8 * SUBS; e++) {
 					x[e] = __builtin_amdgcn_exp2f(
 						__builtin_fmaf(x[e], f.c,
 							       -unit));
 					sm[n].sum += x[e];
 				}
 #pragma unroll
-				for (int e = 0; e < 4; e++)
-					weight[n][e] = pack2<T>(x[2 * e],
-								x[2 * e + 1]);
+				for (int e = 0; e < 4 * SUBS; e++)
+					weight[n][e / 4][e % 4] = pack2<T>(
+						x[2 * e], x[2 * e + 1]);
 			}
 
 			/* Values: O^T += V^T P^T. */
@@ -379,9 +441,10 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 				wait_loads<NI + 1>();
 			else
 				wait_loads<0>();
-			auto value = [&](int d) {
+			auto value = [&](int sub, int d) {
 				if constexpr (sizeof(C) == 2) {
-					const int row = 4 * quarter +
+					const int row = 32 * sub +
+							4 * quarter +
 							(col >> 2);
 					const int piece =
 						(2 * d + ((col & 3) >> 1)) ^
@@ -398,7 +461,7 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 				} else {
 					const int n = col >> 1;
 					const int row =
-						(n < 4 ? 0 : 12) +
+						32 * sub + (n < 4 ? 0 : 12) +
 						4 * quarter + n;
 					const int piece = d ^ N::turn_v(row);
 
@@ -500,13 +563,16 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 				asm volatile("" ::: "memory");
 			}
 #pragma unroll
-			for (int d = 0; d < D / 16; d++) {
-				const u32x4 w = value(d);
+			for (int sub = 0; sub < SUBS; sub++)
 #pragma unroll
-				for (int n = 0; n < NC; n++)
-					out[n][d] = mma16<T>(w, weight[n],
-							     out[n][d]);
-			}
+				for (int d = 0; d < D / 16; d++) {
+					const u32x4 w = value(sub, d);
+#pragma unroll
+					for (int n = 0; n < NC; n++)
+						out[n][d] = mma16<T>(
+							w, weight[n][sub],
+							out[n][d]);
+				}
 			wait_lds();
 			if (more)
 				request(c.v_cache, c.v_page, c.v_slot,
@@ -570,12 +636,9 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 			const float unit = top == -INFINITY ? -INFINITY :
 							      top * f.c - lift;
 
-			if (parts > 1) {
+			if (slot >= 0) {
 				const int64_t at_row =
-					((part * (int64_t)c.batch + b) *
-						 c.kv_heads +
-					 kh) * p.span +
-					r;
+					part_at(p, kh, block, slot) + r;
 				f32x4 *o = (f32x4 *)(p.narrow_out +
 						     at_row * D + d);
 
@@ -602,7 +665,7 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 						 __builtin_amdgcn_logf(sum)) *
 							0.693147181f;
 		}
-		__syncthreads(); /* before the next rows' tiles */
+		__syncthreads(); /* before the next piece's tiles */
 	}
 }
 
@@ -613,7 +676,7 @@ void launch(const nvs_kv &c, const nvs_kv_attend_args &a, const nvs_plan &p,
 	/* Wide rows of 16 bits: half the waves, as their tiles are twice as
 	 * large. */
 	constexpr int W = D * sizeof(C) > 256 ? 2 : 4;
-	const dim3 grid(c.batch * c.kv_heads * p.narrow_parts);
+	const dim3 grid(p.narrow_blocks * c.kv_heads);
 
 	if (p.span == 16)
 		hipLaunchKernelGGL((narrow_kernel<T, C, D, 1, W>), grid,

@@ -86,14 +86,15 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 	const int r0 = (int)block * WIDE_ROWS;
 	const int i0 = r0 / group;
 	const int i1 = min(s.count, (r0 + WIDE_ROWS - 1) / group + 1) - 1;
-	const key_range k =
-		keys_of(c, a.window, s, i0, i1, TILE, WIDE_LEAST, p.wide_parts);
-	const int parts = parts_of(k);
+	key_range k = keys_of(c, a.window, s, i0, i1, TILE);
+	const int per = part_tiles(k, p.wide_parts), parts = parts_of(k, per);
 
 	if (part >= parts)
 		return;
-	const int first = k.first + part * k.per;
-	const int last = min(k.last, first + k.per);
+	k.lo = uniform(k.lo);
+	k.hi = uniform(k.hi);
+	const int first = uniform(k.first + part * per);
+	const int last = uniform(min(k.last, first + per));
 
 	const int *const table = c.table + (int64_t)b * c.table_row;
 	const float vs = sizeof(C) == 1 ? c.v_scale[kh] : 1.f;
@@ -137,7 +138,6 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 		if (real)
 			q[d] = *(const u32x4 *)(src + 16 * d + 8 * half);
 		q[d] = (q[d] ^ f.flip) & f.keep;
-		arrived(q[d]);
 	}
 
 	softmax<T> sm;
@@ -296,6 +296,9 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 			put(0);
 		}
 	}
+#pragma unroll
+	for (int d = 0; d < D / 16; d++)
+		arrived(q[d]);
 	for (int t = first; t < last; t++) {
 		const int n = (t - first) & 1;
 		const char *const k_lds = lds + n * 2 * W::BUFFER;
@@ -542,117 +545,140 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 
 /*
  * Join the parts of rows whose keys were divided.  Rows with one part have
- * their result already.  A row has 256 / ROWS threads: first over the
- * parts, for their weights, then over the dimensions and TP parts at a
- * time.  With many parts a whole block is at work on a row, so that their
- * loads are under way together; with few, a wave is.
+ * their result already.  A row has THREADS threads: first over the parts,
+ * THREADS of them at a time, for their weights, then over the dimensions
+ * and TP parts at a time.  Where a row may have many parts a whole block
+ * is at work on it, so that their loads are under way together; else a
+ * wave is.
  */
-template <typename T, int D, bool NARROW, int ROWS>
+template <typename T, int D, bool NARROW, int THREADS>
 __global__ __launch_bounds__(256) void join_kernel(nvs_kv c,
 						   nvs_kv_attend_args a,
 						   nvs_plan p, int all_rows)
 {
-	constexpr int THREADS = 256 / ROWS;
-	constexpr int PER = ROWS == 1 ? 4 : D / 64 > 4 ? 4 : D / 64;
-	constexpr int TD = D / PER, TP = THREADS / TD;
-	constexpr int MOST = ROWS == 1 ? JOIN_MOST : JOIN_FEW;
+	constexpr int ROWS = 256 / THREADS;
+	constexpr int PER = D / 64; /* dimensions of a thread */
+	constexpr int TP = THREADS / 64;
 	typedef float vec __attribute__((ext_vector_type(PER)));
-	__shared__ vec add[ROWS][TP][TD];
-	__shared__ float scales[ROWS][MOST];
+	__shared__ vec add[ROWS][TP][64];
+	__shared__ float scales[ROWS][THREADS], wave_top[4], wave_sum[4];
 	const int sub = threadIdx.x / THREADS, t = threadIdx.x % THREADS;
-	const int td = t % TD, tp = t / TD;
+	const int td = t % 64, tp = t / 64;
 	const int group = c.heads / c.kv_heads;
 	const int index = blockIdx.x * ROWS + sub;
-	bool mine = index < all_rows;
-	int b = 0, r = 0, head = 0, rows = 0;
-	int64_t at = 0, step = 0; /* of the row in a part, between parts */
+	int b = 0, r = 0, head = 0, parts = 1;
 	sequence s = {};
+	/* Where part n is: the first at at0, the others at + n * step. */
+	int64_t at0 = 0, at = 0, step = 0;
 
-	if (mine) {
-		if (NARROW) {
-			const int item = index / p.joined_rows;
+	if (NARROW && index < all_rows) {
+		const int item = index / p.joined_rows, kh = item % c.kv_heads;
 
-			b = item / c.kv_heads;
-			r = index % p.joined_rows;
-			head = item % c.kv_heads * group + r % group;
-			s = sequence_of(c, b);
-			rows = s.count * group;
-			mine = r < rows && rows <= p.joined_rows;
-			at = (int64_t)item * p.span + r;
-			step = (int64_t)c.batch * c.kv_heads * p.span;
-		} else {
-			head = index % c.heads;
-			b = sequence_at(c, index / c.heads);
-			mine = b >= 0;
-			if (mine) {
-				s = sequence_of(c, b);
-				rows = s.count * group;
-				r = (index / c.heads - s.first) * group +
-				    head % group;
-				mine = r < rows && rows > p.narrow_rows;
-			}
-			at = index;
-			step = (int64_t)c.total * c.heads;
+		b = item / c.kv_heads;
+		r = index % p.joined_rows;
+		head = kh * group + r % group;
+		s = sequence_of(c, b);
+		const int64_t from = p.tiles_at[b], to = p.tiles_at[b + 1];
+		const int64_t tiles = p.tiles_at[c.batch];
+
+		if (from < to && r < s.count * group) {
+			const int64_t used = narrow_used(p, tiles);
+			const int j = narrow_block_of(from, tiles, used);
+
+			parts = narrow_block_of(to - 1, tiles, used) - j + 1;
+			at = part_at(p, kh, j, 0) + r;
+			step = 2 * p.span;
+			/* Not the first piece of its block: the other slot. */
+			at0 = from > j * tiles / used ? at + p.span : at;
 		}
-	}
-	int parts = 1;
+	} else if (index < all_rows) {
+		head = index % c.heads;
+		b = sequence_at(c, index / c.heads);
+		if (b >= 0) {
+			s = sequence_of(c, b);
+			const int rows = s.count * group;
 
-	if (mine) {
-		const int span = NARROW ? p.span : WIDE_ROWS;
-		const int r0 = r / span * span;
+			r = (index / c.heads - s.first) * group + head % group;
+			if (r < rows && rows > p.narrow_rows) {
+				const int r0 = r / WIDE_ROWS * WIDE_ROWS;
+				const key_range k = keys_of(
+					c, a.window, s, r0 / group,
+					min(s.count, (r0 + WIDE_ROWS - 1) /
+								     group +
+							     1) -
+						1,
+					WIDE_TILE);
 
-		parts = parts_of(keys_of(
-			c, a.window, s, r0 / group,
-			min(s.count, (r0 + span - 1) / group + 1) - 1,
-			NARROW ? NARROW_TILE : WIDE_TILE,
-			NARROW ? NARROW_LEAST : WIDE_LEAST,
-			NARROW ? p.narrow_parts : p.wide_parts));
-		mine = parts > 1;
+				parts = parts_of(k,
+						 part_tiles(k, p.wide_parts));
+			}
+		}
+		at = at0 = index;
+		step = (int64_t)c.total * c.heads;
 	}
-	if (ROWS == 1 && !mine)
+	if (THREADS == 256 && parts < 2)
 		return;
-	const f32x2 *sums = (NARROW ? p.narrow_sum : p.wide_sum) + at;
-	const float *outs = (NARROW ? p.narrow_out : p.wide_out) + at * D +
-			    PER * td;
-
-	/* The parts' weights, by the first wave of the row's threads. */
-	float unit = -INFINITY, sum = 0.f;
-
-	if (mine && t < 64) {
-		for (int n = t; n < parts; n += 64)
-			unit = fmaxf(unit, sums[n * step][0]);
+	const f32x2 *sums = NARROW ? p.narrow_sum : p.wide_sum;
+	const float *outs = (NARROW ? p.narrow_out : p.wide_out) + PER * td;
+	auto place = [&](int n) { return n ? at + n * step : at0; };
+	/* Over a row's threads. */
+	auto over = [&](float x, float *waves, auto op) {
 		for (int o = 32; o; o >>= 1)
-			unit = fmaxf(unit, __shfl_xor(unit, o));
-		for (int n = t; n < parts; n += 64) {
-			const f32x2 y = sums[n * step];
+			x = op(x, __shfl_xor(x, o));
+		if (THREADS > 64) {
+			if (td == 0)
+				waves[tp] = x;
+			__syncthreads();
+			x = waves[0];
+			for (int n = 1; n < TP; n++)
+				x = op(x, waves[n]);
+		}
+		return x;
+	};
+	auto larger = [](float x, float y) { return fmaxf(x, y); };
+	auto plus = [](float x, float y) { return x + y; };
+	float unit = -INFINITY, sum = 0.f;
+	vec x = {};
+
+	if (parts < 2)
+		parts = 0; /* a wave that has nothing to do */
+	for (int n = t; n < parts; n += THREADS)
+		unit = fmaxf(unit, sums[place(n)][0]);
+	unit = over(unit, wave_top, larger);
+	for (int n0 = 0; n0 < parts; n0 += THREADS) {
+		const int here = min(parts - n0, THREADS);
+
+		if (THREADS > 64)
+			__syncthreads();
+		if (t < here) {
+			const f32x2 y = sums[place(n0 + t)];
 			const float m =
 				y[0] == -INFINITY ?
 					0.f :
 					__builtin_amdgcn_exp2f(y[0] - unit);
 
-			scales[sub][n] = m;
+			scales[sub][t] = m;
 			sum += m * y[1];
 		}
-		for (int o = 32; o; o >>= 1)
-			sum += __shfl_xor(sum, o);
-	}
-	__syncthreads();
-	vec x = {};
-
-	if (mine) {
+		if (THREADS > 64)
+			__syncthreads();
+		else
+			wait_lds();
 #pragma unroll 8
-		for (int n = tp; n < parts; n += TP)
-			x += scales[sub][n] * *(const vec *)(outs + n * step * D);
+		for (int n = tp; n < here; n += TP)
+			x += scales[sub][n] *
+			     *(const vec *)(outs + place(n0 + n) * D);
 	}
-	if (TP > 1) {
+	sum = over(sum, wave_sum, plus);
+	if (THREADS > 64) {
 		add[sub][tp][td] = x;
 		__syncthreads();
-		if (tp == 0)
-			for (int n = 1; n < TP; n++)
-				x += add[sub][n][td];
-		/* `sum` is the first wave's: TD is at most that. */
+		if (tp)
+			return;
+		for (int n = 1; n < TP; n++)
+			x += add[sub][n][td];
 	}
-	if (!mine || tp)
+	if (!parts)
 		return;
 	const int kh = head / group;
 	const float inv =
@@ -680,12 +706,17 @@ void join(const nvs_kv &c, const nvs_kv_attend_args &a, const nvs_plan &p,
 {
 	const int rows = NARROW ? c.batch * c.kv_heads * p.joined_rows :
 				  c.total * c.heads;
+	/* With 32 rows and parts (one sequence over 120001 keys) a block to
+	 * a row takes 7 us and a wave 16; with 2048 rows of 2 parts, 9 and
+	 * 6. */
+	const int64_t parts = NARROW ? p.narrow_blocks / c.batch :
+				       p.wide_parts;
 
-	if ((NARROW ? p.narrow_parts : p.wide_parts) > JOIN_FEW)
-		hipLaunchKernelGGL((join_kernel<T, D, NARROW, 1>), dim3(rows),
-				   dim3(256), 0, s, c, a, p, rows);
+	if (parts >= 16)
+		hipLaunchKernelGGL((join_kernel<T, D, NARROW, 256>),
+				   dim3(rows), dim3(256), 0, s, c, a, p, rows);
 	else
-		hipLaunchKernelGGL((join_kernel<T, D, NARROW, 4>),
+		hipLaunchKernelGGL((join_kernel<T, D, NARROW, 64>),
 				   dim3((rows + 3) / 4), dim3(256), 0, s, c, a,
 				   p, rows);
 }

@@ -27,30 +27,35 @@
 
 #include "kvdev.h"
 
-constexpr int NARROW_TILE = 32, WIDE_TILE = 64, WIDE_ROWS = 128;
-/* The fewest tiles that are worth a block of their own. */
-constexpr int NARROW_LEAST = 8, WIDE_LEAST = 8;
+constexpr int WIDE_TILE = 64, WIDE_ROWS = 128;
 
-/* The most parts, and the most that one wave joins. */
-constexpr int JOIN_MOST = 1024, JOIN_FEW = 16;
+constexpr int nvs_narrow_tile(int dim, int size)
+{
+	return dim * size < 256 ? 64 : 32;
+}
+
+/* The fewest tiles that are worth a block of their own. */
+constexpr int NARROW_LEAST = 4, WIDE_LEAST = 8;
 
 /* How the work of one call is divided. */
 struct nvs_plan {
 	int narrow_rows; /* sequences with more rows go to the wide kernel */
 	int span;	 /* rows of a narrow block, 16 or 32 */
-	int joined_rows; /* rows of a sequence that narrow parts may have */
-	int narrow_parts, wide_parts; /* blocks that may divide the keys */
-	int wide_blocks;	      /* blocks of rows, for one cached head */
+	int joined_rows; /* rows of a sequence that may be divided there */
+	int narrow_blocks; /* narrow blocks for one cached head */
+	int wide_blocks;   /* blocks of rows, for one cached head */
+	int wide_parts;	   /* wide blocks that may divide one's keys */
+	int cover; /* the launch that sees to rows of no sequence: 1 narrow,
+		      2 wide */
 	uint64_t page_magic; /* key / page_size = key * magic >> shift */
 	int page_shift;
 	int near_slots; /* a tile's rows lie within 31 bits of each other */
-	int cover; /* the launch that sees to rows of no sequence: 1 narrow,
-		      2 wide */
 	/* Results and (log2 of the weights' unit, sum of the weights in it)
-	 * of parts: [part][sequence][cached head][row of span] of narrow
-	 * blocks, [part][row][head] of wide ones. */
+	 * of parts: of narrow blocks by part_at(), of wide ones by [part]
+	 * [row][head]. */
 	float *narrow_out, *wide_out;
 	f32x2 *narrow_sum, *wide_sum;
+	int64_t *tiles_at; /* [batch + 1]: the sequences' first tiles */
 };
 
 template <typename T, typename C>
@@ -63,39 +68,173 @@ template <typename T>
 hipError_t nvs_join(const nvs_kv &c, const nvs_kv_attend_args &a,
 		    const nvs_plan &p, bool narrow, hipStream_t s);
 
-/* The keys [lo, hi) that some of the tokens [i0, i1] of s see, and how many
- * tiles of them a part has. */
+/* The keys [lo, hi) that some of the tokens [i0, i1] of s see, and their
+ * tiles. */
 struct key_range {
-	int lo, hi;	 /* keys */
-	int first, last; /* tiles */
-	int per;	 /* tiles of a part */
+	int lo, hi;
+	int first, last;
 };
 
 __device__ __forceinline__ key_range keys_of(const nvs_kv &c, int window,
 					     const sequence &s, int i0, int i1,
-					     int tile, int least, int parts)
+					     int tile)
 {
 	const int64_t capacity = (int64_t)c.per_seq * c.page_size;
 	const int64_t hi = min(s.pos + i1 + 1, capacity);
 	const int64_t lo = window > 0 ? s.pos + i0 + 1 - window : 0;
 	key_range k;
 
-	k.lo = uniform((int)min(max(lo, (int64_t)0), capacity));
-	k.hi = uniform((int)max(hi, (int64_t)0));
-	if (k.hi <= k.lo) {
-		k.lo = k.hi = k.first = k.last = 0;
-		k.per = 1;
-		return k;
-	}
+	k.lo = (int)min(max(lo, (int64_t)0), capacity);
+	k.hi = (int)max(hi, (int64_t)0);
+	if (k.hi <= k.lo)
+		k.lo = k.hi = 0;
 	k.first = k.lo / tile;
 	k.last = (k.hi + tile - 1) / tile;
-	k.per = max(least, (k.last - k.first + parts - 1) / parts);
 	return k;
 }
 
-__device__ __forceinline__ int parts_of(const key_range &k)
+/* The wide kernel divides the tiles of a block of rows evenly: how many go
+ * to a part, and how many parts there are. */
+__device__ __forceinline__ int part_tiles(const key_range &k, int parts)
 {
-	return max(1, (k.last - k.first + k.per - 1) / k.per);
+	return max(WIDE_LEAST, (k.last - k.first + parts - 1) / parts);
+}
+
+__device__ __forceinline__ int parts_of(const key_range &k, int per)
+{
+	return max(1, (k.last - k.first + per - 1) / per);
+}
+
+/*
+ * The narrow kernel lays the tiles of all its sequences end to end and
+ * gives each of its blocks (for a cached head) the same number, however
+ * unlike the sequences are: a block then has the end of one sequence, some
+ * whole ones and the beginning of another, or a part of a long one.  Each
+ * of its first and last pieces that is not a whole sequence goes to a slot
+ * of the block's for the join.
+ */
+__device__ __forceinline__ key_range narrow_keys(const nvs_kv &c,
+						 const nvs_kv_attend_args &a,
+						 const nvs_plan &p,
+						 const sequence &s, int tile)
+{
+	return keys_of(c, a.window, s, 0, s.count - 1, tile);
+}
+
+/* A sequence's tiles there: one at least where it has rows, as these have
+ * a result; none where it is not for the narrow kernel or has more rows
+ * than the caller said. */
+__device__ __forceinline__ int narrow_tiles(const nvs_kv &c, const nvs_plan &p,
+					    const sequence &s,
+					    const key_range &k)
+{
+	const int64_t rows = (int64_t)s.count * (c.heads / c.kv_heads);
+
+	return rows == 0 || rows > p.joined_rows ?
+		       0 :
+		       max(1, k.last - k.first);
+}
+
+/* How many blocks there are enough tiles for. */
+__device__ __forceinline__ int64_t narrow_used(const nvs_plan &p,
+					       int64_t tiles)
+{
+	return min((int64_t)p.narrow_blocks,
+		   max(tiles / NARROW_LEAST, (int64_t)1));
+}
+
+/* The block that has tile x of `tiles`; block j of `used` begins with tile
+ * j * tiles / used. */
+__device__ __forceinline__ int narrow_block_of(int64_t x, int64_t tiles,
+					       int64_t used)
+{
+	return (int)(((x + 1) * used - 1) / tiles);
+}
+
+__device__ __forceinline__ int64_t part_at(const nvs_plan &p, int kh,
+					   int block, int slot)
+{
+	return (((int64_t)kh * p.narrow_blocks + block) * 2 + slot) * p.span;
+}
+
+struct share {
+	int64_t from, to; /* tiles */
+	int b;		  /* the sequence of tile `from`, or one before it */
+	int64_t b_from;	  /* its first tile */
+};
+
+__device__ __forceinline__ share share_of(const nvs_kv &c,
+					  const nvs_kv_attend_args &a,
+					  const nvs_plan &p, int tile,
+					  int block, bool leave)
+{
+	const int lane = threadIdx.x & 63;
+	/* The tiles of sequence b0 + lane, and with those of the 63 before
+	 * it: all the card's memory has fewer than 32 bits of them. */
+	auto scan = [&](int b0, unsigned &own) {
+		own = 0;
+		if (b0 + lane < c.batch) {
+			const sequence s = sequence_of(c, b0 + lane);
+
+			own = narrow_tiles(c, p, s,
+					   narrow_keys(c, a, p, s, tile));
+		}
+		unsigned sum = own;
+
+		if (c.batch > 1)
+#pragma unroll
+			for (int o = 1; o < 64; o <<= 1) {
+				const unsigned x = __shfl_up(sum, o);
+
+				sum += lane >= o ? x : 0;
+			}
+		return sum;
+	};
+	int64_t tiles = 0;
+	unsigned sum = 0, own = 0;
+
+	for (int b0 = 0; b0 < c.batch; b0 += 64) {
+		sum = scan(b0, own);
+		if (leave && p.tiles_at && b0 + lane < c.batch)
+			p.tiles_at[b0 + lane] = tiles + sum - own;
+		tiles += (unsigned)__builtin_amdgcn_readlane(
+			sum, c.batch > 1 ? 63 : 0);
+	}
+	if (leave && p.tiles_at && lane == 0)
+		p.tiles_at[c.batch] = tiles;
+
+	const int64_t used = narrow_used(p, tiles);
+	share m = {};
+
+	if (block >= used || tiles == 0)
+		return m;
+	m.from = block * tiles / used;
+	m.to = (block + 1) * tiles / used;
+	/* The last 64 sequences that begin no later, then the last one. */
+	int64_t before = 0;
+
+	for (int b0 = 0; c.batch > 1 && b0 < c.batch; b0 += 64) {
+		if (c.batch > 64)
+			sum = scan(b0, own);
+		const int64_t all =
+			(unsigned)__builtin_amdgcn_readlane(sum, 63);
+
+		if (before + all > m.from) {
+			const uint64_t later =
+				__ballot(before + sum > m.from);
+			const int n = __builtin_ctzll(later);
+
+			m.b = b0 + n;
+			m.b_from = before + (unsigned)__shfl(sum - own, n);
+			break;
+		}
+		before += all;
+	}
+	m.from = uniform64(m.from);
+	m.to = uniform64(m.to);
+	m.b = uniform(m.b);
+	m.b_from = uniform64(m.b_from);
+	return m;
 }
 
 /* The number in its sequence of the page of a position. */

@@ -291,14 +291,23 @@ nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, void *work,
 	p.span = most_rows > 32 || most_rows <= 16 ? 16 : 32;
 	p.narrow_rows = most_rows <= 32 ? 0x7fffffff : c.starts ? 16 : 0;
 	p.joined_rows = (int)(most_rows < p.span ? most_rows : p.span);
-	p.narrow_parts = p.wide_parts = 1;
+	p.narrow_blocks = p.narrow_rows ? 1 : 0;
+	p.wide_parts = 1;
 	if (p.narrow_rows && p.joined_rows) {
-		const int64_t items = (int64_t)c.batch * c.kv_heads;
-		const int64_t want = ceil_div(1024, items);
-		const int64_t most =
-			ceil_div(ceil_div(keys, NARROW_TILE), NARROW_LEAST);
+		/* As many blocks as the card holds at a time (2 a CU, 4 of
+		 * the smallest rows): all begin and end together.  Twice as
+		 * many take 390 us where these take 383, for 64 tokens over
+		 * 8192 keys each, and 39 where these take 33, over 500. */
+		const int size = c.cache_type == NVS_KV_E4M3 ? 1 : 2;
+		const int64_t tile = nvs_narrow_tile(c.dim, size);
+		const int64_t most = ceil_div(
+			c.batch * ceil_div(keys, tile), NARROW_LEAST);
+		const int64_t want = (c.dim * size < 128 ? 1024 : 512) /
+				     c.kv_heads;
 
-		p.narrow_parts = (int)(want < most ? want : most);
+		p.narrow_blocks = (int)(most < want ? most :
+					want > 1   ? want :
+						     1);
 	}
 	if (most_rows > 32) {
 		p.wide_blocks =
@@ -316,8 +325,8 @@ nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, void *work,
 		p.cover = p.narrow_rows ? 1 : 2;
 
 	/* The parts' results, narrow before wide. */
-	const int64_t narrow = p.narrow_parts > 1 ?
-				       (int64_t)p.narrow_parts * c.batch *
+	const int64_t narrow = p.narrow_blocks > 1 ?
+				       (int64_t)p.narrow_blocks * 2 *
 					       c.kv_heads * p.span :
 				       0;
 	const int64_t wide = p.wide_parts > 1 ? (int64_t)p.wide_parts *
@@ -329,6 +338,10 @@ nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, void *work,
 	p.narrow_sum = (f32x2 *)(p.wide_out + wide * c.dim);
 	p.wide_sum = p.narrow_sum + narrow;
 	bytes = (narrow + wide) * (c.dim * 4 + 8);
+	if (narrow) {
+		p.tiles_at = (int64_t *)(p.wide_sum + wide);
+		bytes += (c.batch + 1ll) * 8;
+	}
 	return p;
 }
 
@@ -342,7 +355,7 @@ int launch_attend(const nvs_kv &c, const nvs_kv_attend_args &a,
 		e = nvs_narrow<T, C>(c, a, p, s);
 	if (e == hipSuccess && p.wide_blocks)
 		e = nvs_wide<T, C>(c, a, p, s);
-	if (e == hipSuccess && p.narrow_parts > 1)
+	if (e == hipSuccess && p.narrow_blocks > 1)
 		e = nvs_join<T>(c, a, p, true, s);
 	if (e == hipSuccess && p.wide_parts > 1)
 		e = nvs_join<T>(c, a, p, false, s);
@@ -406,7 +419,7 @@ int nvs_kv_attend(const nvs_kv *c, const nvs_kv_attend_args *a, void *work,
 	const nvs_plan p = plan_of(*c, *a, work, bytes);
 
 	if ((bytes && (!work || !aligned(work, 16))) ||
-	    too_large((int64_t)c->batch * c->kv_heads * p.narrow_parts, 256) ||
+	    too_large((int64_t)p.narrow_blocks * c->kv_heads, 256) ||
 	    too_large((int64_t)p.wide_blocks * c->kv_heads * p.wide_parts,
 		      256))
 		return (int)hipErrorInvalidValue;

@@ -54,6 +54,12 @@ __device__ __forceinline__ int uniform(int x)
 	return __builtin_amdgcn_readfirstlane(x);
 }
 
+__device__ __forceinline__ int64_t uniform64(int64_t x)
+{
+	return (int64_t)(((uint64_t)(unsigned)uniform((int)(x >> 32)) << 32) |
+			 (unsigned)uniform((int)x));
+}
+
 /* Two numbers rounded to nearest, ties to even. */
 template <typename T>
 __device__ __forceinline__ unsigned pack2(float a, float b)
