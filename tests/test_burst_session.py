@@ -1,0 +1,74 @@
+"""infer_burst --model session: the cache's operators as a client calls
+them, on the CPU and, with -m gpu, on an MI355X."""
+
+from __future__ import annotations
+
+import json
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from nvshare_amd.workloads import infer_burst
+from nvshare_amd.workloads.session import Sessions
+
+
+def run(*args):
+    r = subprocess.run(
+        [sys.executable, "-m", "nvshare_amd.workloads.infer_burst",
+         "--model", "session", "--think-s", "0.05", *args],
+        capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0, r.stderr[-3000:]
+    assert "PASS" in r.stdout
+    return json.loads(r.stdout.strip().splitlines()[-1])
+
+
+def test_session_cpu():
+    res = run("--device", "cpu", "--batch", "2", "--bursts", "2",
+              "--infers-per-burst", "3", "--prompt", "9", "--layers", "2",
+              "--heads", "4", "--kv-heads", "2", "--head-dim", "64",
+              "--page", "16")
+    assert res["infers"] == 8 and res["tokens"] == 2 * 2 * 12
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_session_notices_a_changed_cache(cache):
+    m = Sessions(2, 40, layers=1, heads=2, kv_heads=1, dim=64, page=16,
+                 cache=cache, device="cpu")
+    m.step(19)
+    before = m.fingerprint()
+    m.check()
+    page = int(m.table[1, 1])
+    m.caches[0].v.view(torch.uint8)[page, 5] ^= 1  # behind the last token
+    assert m.fingerprint() == before
+    m.caches[0].v.view(torch.uint8)[page, 2] ^= 1
+    assert m.fingerprint() != before
+
+
+def test_session_notices_a_wrong_answer():
+    m = Sessions(1, 40, layers=1, heads=2, kv_heads=1, dim=64, page=16,
+                 device="cpu")
+    m.step(30)
+    m.answer[2][3, 1, 7] += 0.5
+    with pytest.raises(SystemExit):
+        m.check()
+
+
+def test_other_models_stay(capsys):
+    infer_burst.main(["--device", "cpu", "--model", "tiny", "--batch", "1",
+                      "--image", "32", "--bursts", "1",
+                      "--infers-per-burst", "1", "--think-s", "0"])
+    assert json.loads(capsys.readouterr().out.splitlines()[-1])[
+        "infers"] == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_session_gpu(cache, dtype):
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU here")
+    res = run("--batch", "4", "--bursts", "2", "--infers-per-burst", "10",
+              "--prompt", "300", "--cache", cache, "--dtype", dtype)
+    assert res["infers"] == 22 and res["tokens"] == 4 * 2 * 310
