@@ -1,7 +1,6 @@
 /*
  * nvshare-amd: arguments of the paged key/value cache's kernels
- * (libnvshare_hiputil.so).  nvshare_amd/hiputil.py lays them out by the
- * same members.  Strides are in values, not bytes.
+ * (libnvshare_hiputil.so).  Strides are in values, not bytes.
  */
 #ifndef NVS_KVCACHE_H
 #define NVS_KVCACHE_H

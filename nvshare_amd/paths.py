@@ -24,7 +24,8 @@ class Artifacts:
     ctl: Path
     stub_dir: Path        # directory holding the CPU stub libamdhip64
     hipclient: Path
-    hiputil: Path         # gfx950 utility kernel library (may not exist)
+    hiputil: Path         # gfx950 kernel library (may not exist)
+    kvbind: Path          # torch's way into its cache kernels (likewise)
 
     def built(self) -> bool:
         return (
@@ -44,6 +45,7 @@ def artifacts() -> Artifacts:
         stub_dir=base,
         hipclient=base / "hipclient",
         hiputil=HIP_BUILD_DIR / "libnvshare_hiputil.so",
+        kvbind=HIP_BUILD_DIR / "_kvbind.so",
     )
 
 
@@ -64,4 +66,13 @@ def ensure_built() -> Artifacts:
         raise RuntimeError(
             "nvshare-amd native components missing; run `make -C src`"
         )
+    return art
+
+
+def ensure_kernels() -> Artifacts:
+    """Build the gfx950 kernels (hipcc, a minute) unless they are there."""
+    art = artifacts()
+    if not (art.hiputil.exists() and art.kvbind.exists()):
+        subprocess.run(["make", "-C", str(REPO_ROOT / "hip"), "-s", "-j4"],
+                       check=True)
     return art

@@ -10,8 +10,14 @@ import sys
 import pytest
 import torch
 
+from nvshare_amd.paths import ensure_kernels
 from nvshare_amd.workloads import infer_burst
 from nvshare_amd.workloads.session import Sessions
+
+
+@pytest.fixture(scope="module", autouse=True)
+def kernels():
+    ensure_kernels()
 
 
 def run(*args):

@@ -22,9 +22,15 @@ import pytest
 import torch
 
 from nvshare_amd.kvcache import PagedCache, append, attend, rotation_table
+from nvshare_amd.paths import ensure_kernels
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 E4M3 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module", autouse=True)
+def kernels():
+    ensure_kernels()
 
 
 @pytest.fixture(params=DEVICES)
@@ -881,45 +887,16 @@ def test_refusals_of_layouts(gpu):
                                            64, 64, device="cpu")))
 
 
-def test_entry_refuses_what_the_kernels_cannot_take():
+def test_entries_refuse_what_the_kernels_cannot_take():
     """The C entries check again: no GPU is needed to be refused."""
-    from nvshare_amd import hiputil
+    import ctypes
 
     from nvshare_amd.paths import artifacts
 
-    if not artifacts().hiputil.exists():
-        pytest.skip("libnvshare_hiputil.so is not built")
-    lib = hiputil.load()
-    kv, app, att = (bytes(x.size) for x in (
-        hiputil.KV_CACHE, hiputil.KV_APPEND, hiputil.KV_ATTEND))
-    for call in (lambda: lib.kv_append(kv, app, 0),
-                 lambda: lib.kv_attend(kv, att, 0, 0),
-                 lambda: lib.kv_attend_work(kv, att)):
-        with pytest.raises(RuntimeError, match="hipError_t=1"):
-            call()
-
-
-def test_structures_match_the_header():
-    """hiputil's structures have the header's members in its order."""
-    import re
-
-    from nvshare_amd import hiputil
-    from nvshare_amd.paths import REPO_ROOT
-
-    text = (REPO_ROOT / "hip" / "kvcache.h").read_text()
-    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
-    codes = {"int64_t": "q", "int": "i", "float": "f"}
-    for struct, packed in (("nvs_kv", hiputil.KV_CACHE),
-                           ("nvs_kv_append_args", hiputil.KV_APPEND),
-                           ("nvs_kv_attend_args", hiputil.KV_ATTEND)):
-        body = re.search(r"struct %s \{(.*?)\};" % struct, text, re.S)[1]
-        names, code = [], ""
-        for line in body.split(";"):
-            m = re.match(r"\s*(?:const )?(\w+) (.*)", line, re.S)
-            if m:
-                for name in m[2].split(","):
-                    name = name.strip()
-                    code += "P" if name.startswith("*") else codes[m[1]]
-                    names.append(name.lstrip("*"))
-        assert packed.names == names
-        assert packed.format == "@" + code + "0P"
+    lib = ctypes.CDLL(str(artifacts().hiputil))
+    lib.nvs_kv_attend_work.restype = ctypes.c_int64
+    zeros = bytes(512)
+    assert lib.nvs_kv_append(zeros, zeros, None) == 1
+    assert lib.nvs_kv_attend(zeros, zeros, None, None) == 1
+    assert lib.nvs_kv_attend_work(zeros, zeros) == -1
+    assert lib.nvs_kv_append(None, None, None) == 1
