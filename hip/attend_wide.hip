@@ -87,13 +87,14 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 	const int i0 = r0 / group;
 	const int i1 = min(s.count, (r0 + WIDE_ROWS - 1) / group + 1) - 1;
 	key_range k = keys_of(c, a.window, s, i0, i1, TILE);
-	const int per = part_tiles(k, p.wide_parts), parts = parts_of(k, per);
+	const int parts = parts_of(k, p.wide_parts);
+	const int per = (k.last - k.first + parts - 1) / parts;
 
 	if (part >= parts)
 		return;
 	k.lo = uniform(k.lo);
 	k.hi = uniform(k.hi);
-	const int first = uniform(k.first + part * per);
+	const int first = uniform(min(k.last, k.first + part * per));
 	const int last = uniform(min(k.last, first + per));
 
 	const int *const table = c.table + (int64_t)b * c.table_row;
@@ -394,12 +395,14 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 			/* Keys: S^T = K Q^T. */
 			f32x16 score[2];
 #pragma unroll
-			for (int h = 0; h < 2; h++) {
+			for (int h = 0; h < 2; h++)
 #pragma unroll
 				for (int e = 0; e < 16; e++)
 					score[h][e] = 0.f;
 #pragma unroll
-				for (int d = 0; d < D / 16; d++) {
+			for (int d = 0; d < D / 16; d++)
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
 					const int row = 32 * h + col;
 					const u32x4 w = *(
 						const u32x4 *)(k_lds +
@@ -411,8 +414,6 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 
 					score[h] = mma32<T>(w, q[d], score[h]);
 				}
-			}
-
 			/* Weights. */
 			if (valid != ~0ull || key0 + TILE - 1 > all ||
 			    key0 < any_low) {
@@ -545,27 +546,25 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 
 /*
  * Join the parts of rows whose keys were divided.  Rows with one part have
- * their result already.  A row has THREADS threads: first over the parts,
- * THREADS of them at a time, for their weights, then over the dimensions
- * and TP parts at a time.  Where a row may have many parts a whole block
- * is at work on it, so that their loads are under way together; else a
- * wave is.
+ * their result already.  A row has WAVES waves, each of them with every
+ * WAVES-th part, several at a time so that their loads are under way
+ * together.
  */
-template <typename T, int D, bool NARROW, int THREADS>
+template <typename T, int D, bool NARROW, int WAVES>
 __global__ __launch_bounds__(256) void join_kernel(nvs_kv c,
 						   nvs_kv_attend_args a,
 						   nvs_plan p, int all_rows)
 {
-	constexpr int ROWS = 256 / THREADS;
-	constexpr int PER = D / 64; /* dimensions of a thread */
-	constexpr int TP = THREADS / 64;
+	constexpr int PER = D / 64; /* dimensions of a lane */
+	constexpr int MANY = WAVES > 1 ? 8 : 4; /* parts at a time */
 	typedef float vec __attribute__((ext_vector_type(PER)));
-	__shared__ vec add[ROWS][TP][64];
-	__shared__ float scales[ROWS][THREADS], wave_top[4], wave_sum[4];
-	const int sub = threadIdx.x / THREADS, t = threadIdx.x % THREADS;
-	const int td = t % 64, tp = t / 64;
+	__shared__ vec add[4][64];
+	__shared__ float units[4], sums[4];
+	const int lane = threadIdx.x % 64;
+	const int wave = uniform(threadIdx.x / 64);
 	const int group = c.heads / c.kv_heads;
-	const int index = blockIdx.x * ROWS + sub;
+	const int index = (blockIdx.x * 4 + wave) / WAVES;
+	const int tp = wave % WAVES;
 	int b = 0, r = 0, head = 0, parts = 1;
 	sequence s = {};
 	/* Where part n is: the first at at0, the others at + n * step. */
@@ -577,10 +576,10 @@ __global__ __launch_bounds__(256) void join_kernel(nvs_kv c,
 		b = item / c.kv_heads;
 		r = index % p.joined_rows;
 		head = kh * group + r % group;
-		s = sequence_of(c, b);
 		const int64_t from = p.tiles_at[b], to = p.tiles_at[b + 1];
 		const int64_t tiles = p.tiles_at[c.batch];
 
+		s = sequence_of(c, b);
 		if (from < to && r < s.count * group) {
 			const int64_t used = narrow_used(p, tiles);
 			const int j = narrow_block_of(from, tiles, used);
@@ -601,90 +600,96 @@ __global__ __launch_bounds__(256) void join_kernel(nvs_kv c,
 			r = (index / c.heads - s.first) * group + head % group;
 			if (r < rows && rows > p.narrow_rows) {
 				const int r0 = r / WIDE_ROWS * WIDE_ROWS;
-				const key_range k = keys_of(
-					c, a.window, s, r0 / group,
-					min(s.count, (r0 + WIDE_ROWS - 1) /
-								     group +
-							     1) -
-						1,
-					WIDE_TILE);
 
-				parts = parts_of(k,
-						 part_tiles(k, p.wide_parts));
+				parts = parts_of(
+					keys_of(c, a.window, s, r0 / group,
+						min(s.count,
+						    (r0 + WIDE_ROWS - 1) /
+								    group +
+							    1) -
+							1,
+						WIDE_TILE),
+					p.wide_parts);
 			}
 		}
 		at = at0 = index;
 		step = (int64_t)c.total * c.heads;
 	}
-	if (THREADS == 256 && parts < 2)
-		return;
-	const f32x2 *sums = NARROW ? p.narrow_sum : p.wide_sum;
-	const float *outs = (NARROW ? p.narrow_out : p.wide_out) + PER * td;
-	auto place = [&](int n) { return n ? at + n * step : at0; };
-	/* Over a row's threads. */
-	auto over = [&](float x, float *waves, auto op) {
-		for (int o = 32; o; o >>= 1)
-			x = op(x, __shfl_xor(x, o));
-		if (THREADS > 64) {
-			if (td == 0)
-				waves[tp] = x;
-			__syncthreads();
-			x = waves[0];
-			for (int n = 1; n < TP; n++)
-				x = op(x, waves[n]);
-		}
-		return x;
-	};
-	auto larger = [](float x, float y) { return fmaxf(x, y); };
-	auto plus = [](float x, float y) { return x + y; };
+	parts = uniform(parts);
+	if (parts < 2)
+		return; /* with WAVES = 4 the whole block */
+	const f32x2 *const part_sum = NARROW ? p.narrow_sum : p.wide_sum;
+	const float *const part_out = (NARROW ? p.narrow_out : p.wide_out) +
+				      PER * lane;
 	float unit = -INFINITY, sum = 0.f;
 	vec x = {};
+	auto weigh = [](float u, float top) {
+		return u == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(u - top);
+	};
 
-	if (parts < 2)
-		parts = 0; /* a wave that has nothing to do */
-	for (int n = t; n < parts; n += THREADS)
-		unit = fmaxf(unit, sums[place(n)][0]);
-	unit = over(unit, wave_top, larger);
-	for (int n0 = 0; n0 < parts; n0 += THREADS) {
-		const int here = min(parts - n0, THREADS);
+	for (int n0 = tp; n0 < parts; n0 += MANY * WAVES) {
+		f32x2 y[MANY];
+		vec v[MANY];
+		float top = unit;
 
-		if (THREADS > 64)
-			__syncthreads();
-		if (t < here) {
-			const f32x2 y = sums[place(n0 + t)];
-			const float m =
-				y[0] == -INFINITY ?
-					0.f :
-					__builtin_amdgcn_exp2f(y[0] - unit);
+#pragma unroll
+		for (int i = 0; i < MANY; i++) {
+			const int n = n0 + i * WAVES;
+			const int m = min(n, parts - 1);
+			const int64_t place = m ? at + m * step : at0;
 
-			scales[sub][t] = m;
-			sum += m * y[1];
+			y[i] = part_sum[place];
+			v[i] = *(const vec *)(part_out + place * D);
+			if (n >= parts)
+				y[i][0] = -INFINITY;
 		}
-		if (THREADS > 64)
-			__syncthreads();
-		else
-			wait_lds();
-#pragma unroll 8
-		for (int n = tp; n < here; n += TP)
-			x += scales[sub][n] *
-			     *(const vec *)(outs + place(n0 + n) * D);
+#pragma unroll
+		for (int i = 0; i < MANY; i++)
+			top = fmaxf(top, y[i][0]);
+		const float keep = weigh(unit, top);
+
+		sum *= keep;
+		x *= keep;
+#pragma unroll
+		for (int i = 0; i < MANY; i++) {
+			const float m = weigh(y[i][0], top);
+
+			/* A part that saw no key has weight 0 and zeros. */
+			sum += m * y[i][1];
+			x += m * v[i];
+		}
+		unit = top;
 	}
-	sum = over(sum, wave_sum, plus);
-	if (THREADS > 64) {
-		add[sub][tp][td] = x;
+	if (WAVES > 1) {
+		add[wave][lane] = x;
+		if (lane == 0) {
+			units[wave] = unit;
+			sums[wave] = sum;
+		}
 		__syncthreads();
 		if (tp)
 			return;
-		for (int n = 1; n < TP; n++)
-			x += add[sub][n][td];
+		float top = unit;
+
+		for (int n = 1; n < WAVES; n++)
+			top = fmaxf(top, units[n]);
+		const float keep = weigh(unit, top);
+
+		sum *= keep;
+		x *= keep;
+		for (int n = 1; n < WAVES; n++) {
+			const float m = weigh(units[n], top);
+
+			sum += m * sums[n];
+			x += m * add[n][lane];
+		}
+		unit = top;
 	}
-	if (!parts)
-		return;
 	const int kh = head / group;
 	const float inv =
 		sum == 0.f ? 0.f : (c.v_scale ? c.v_scale[kh] : 1.f) / sum;
 	const int64_t row = s.first + r / group;
-	T *o = (T *)a.out + row * a.out_row + head * a.out_head + PER * td;
+	T *o = (T *)a.out + row * a.out_row + head * a.out_head + PER * lane;
 
 	if constexpr (PER == 1)
 		*o = (T)(x[0] * inv);
@@ -693,7 +698,7 @@ __global__ __launch_bounds__(256) void join_kernel(nvs_kv c,
 		for (int e = 0; e < PER; e += 2)
 			*(unsigned *)(o + e) =
 				pack2<T>(x[e] * inv, x[e + 1] * inv);
-	if (a.lse && td == 0)
+	if (a.lse && lane == 0)
 		a.lse[row * c.heads + head] =
 			sum == 0.f ? -INFINITY :
 				     (unit + __builtin_amdgcn_logf(sum)) *
@@ -713,10 +718,10 @@ void join(const nvs_kv &c, const nvs_kv_attend_args &a, const nvs_plan &p,
 				       p.wide_parts;
 
 	if (parts >= 16)
-		hipLaunchKernelGGL((join_kernel<T, D, NARROW, 256>),
+		hipLaunchKernelGGL((join_kernel<T, D, NARROW, 4>),
 				   dim3(rows), dim3(256), 0, s, c, a, p, rows);
 	else
-		hipLaunchKernelGGL((join_kernel<T, D, NARROW, 64>),
+		hipLaunchKernelGGL((join_kernel<T, D, NARROW, 1>),
 				   dim3((rows + 3) / 4), dim3(256), 0, s, c, a,
 				   p, rows);
 }

@@ -35,7 +35,7 @@ constexpr int nvs_narrow_tile(int dim, int size)
 }
 
 /* The fewest tiles that are worth a block of their own. */
-constexpr int NARROW_LEAST = 4, WIDE_LEAST = 8;
+constexpr int NARROW_LEAST = 4, WIDE_LEAST = 16;
 
 /* How the work of one call is divided. */
 struct nvs_plan {
@@ -93,16 +93,11 @@ __device__ __forceinline__ key_range keys_of(const nvs_kv &c, int window,
 	return k;
 }
 
-/* The wide kernel divides the tiles of a block of rows evenly: how many go
- * to a part, and how many parts there are. */
-__device__ __forceinline__ int part_tiles(const key_range &k, int parts)
+/* The wide kernel divides the tiles of a block of rows evenly between so
+ * many parts. */
+__device__ __forceinline__ int parts_of(const key_range &k, int most)
 {
-	return max(WIDE_LEAST, (k.last - k.first + parts - 1) / parts);
-}
-
-__device__ __forceinline__ int parts_of(const key_range &k, int per)
-{
-	return max(1, (k.last - k.first + per - 1) / per);
+	return max(1, min(most, (k.last - k.first) / WIDE_LEAST));
 }
 
 /*

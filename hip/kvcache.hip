@@ -314,12 +314,19 @@ nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, void *work,
 			(int)(c.starts ? c.total * group / WIDE_ROWS + c.batch :
 					 c.batch *
 						 ceil_div(most_rows, WIDE_ROWS));
-		const int64_t want = 512 / ((int64_t)p.wide_blocks *
-					    c.kv_heads);
+		/* Two blocks a CU.  A block of rows sees no more keys than
+		 * its window and its own tokens. */
+		const int64_t want =
+			512 / ((int64_t)p.wide_blocks * c.kv_heads);
+		const int64_t seen = a.window + WIDE_ROWS / group + 1;
 		const int64_t most =
-			ceil_div(ceil_div(keys, WIDE_TILE), WIDE_LEAST);
+			ceil_div(a.window > 0 && seen < keys ? seen : keys,
+				 WIDE_TILE) /
+			WIDE_LEAST;
 
-		p.wide_parts = (int)(want < 1 ? 1 : want < most ? want : most);
+		p.wide_parts = (int)(want < most ? want : most);
+		if (p.wide_parts < 1)
+			p.wide_parts = 1;
 	}
 	if (c.starts)
 		p.cover = p.narrow_rows ? 1 : 2;
