@@ -9,6 +9,7 @@
  */
 #include <torch/extension.h>
 
+#include <cmath>
 #include <limits>
 #include <optional>
 #include <sstream>
@@ -73,11 +74,27 @@ void check_strides(const char *name, const Tensor &t, int64_t step)
 	bool fine = t.stride(-1) == 1 && (uintptr_t)t.data_ptr() % 16 == 0;
 
 	for (int64_t d = 0; d + 1 < t.dim(); d++)
-		fine &= t.stride(d) % step == 0;
+		fine &= t.size(d) == 1 || t.stride(d) % step == 0;
 	if (!fine)
 		refuse(name, ": values of a head are not contiguous at 16 bytes"
 			     " (strides ",
 		       t.strides(), ")");
+}
+
+/* A stride that is never taken is none. */
+int64_t step(const Tensor &t, int64_t d)
+{
+	return t.size(d) == 1 ? 0 : t.stride(d);
+}
+
+/* Nothing in `t`, which is written, is in two places. */
+void check_distinct(const char *name, const Tensor &t)
+{
+	for (int64_t d = 0; d < t.dim(); d++)
+		if (t.size(d) > 1 && t.stride(d) == 0)
+			refuse(name, ": an expanded tensor cannot be written "
+				     "to (strides ",
+			       t.strides(), ")");
 }
 
 void check_index(const char *name, const Tensor &t, int64_t n,
@@ -171,13 +188,13 @@ nvs_kv describe(const Tensor &ck, const Tensor &cv, const Maybe &k_scale,
 	c.table = (const int *)table.data_ptr();
 	c.lens = (const int *)lens.data_ptr();
 	c.starts = (const int *)at_of(starts);
-	c.table_row = table.stride(0);
-	c.k_page = ck.stride(0);
-	c.k_slot = ck.stride(1);
-	c.k_head = ck.stride(2);
-	c.v_page = cv.stride(0);
-	c.v_slot = cv.stride(1);
-	c.v_head = cv.stride(2);
+	c.table_row = step(table, 0);
+	c.k_page = step(ck, 0);
+	c.k_slot = step(ck, 1);
+	c.k_head = step(ck, 2);
+	c.v_page = step(cv, 0);
+	c.v_slot = step(cv, 1);
+	c.v_head = step(cv, 2);
 	c.type = type;
 	c.cache_type = e4m3 ? NVS_KV_E4M3 : type;
 	c.batch = (int)batch;
@@ -252,16 +269,21 @@ Maybe append(const Tensor &ck, const Tensor &cv, const Maybe &k_scale,
 			       " positions, the table names ",
 			       (int64_t)c.per_seq * c.page_size);
 		a.rotation = (const float *)rotation->data_ptr();
-		a.rotation_row = rotation->stride(0);
+		a.rotation_row = step(*rotation, 0);
 		a.rotary = (int)rotary;
 		a.interleaved = interleaved;
 	}
-	forward_only({ &k, &v, q ? &*q : nullptr, q_out ? &*q_out : nullptr });
+	forward_only({ &ck, &cv, &k, &v, q ? &*q : nullptr,
+		       q_out ? &*q_out : nullptr });
+	check_distinct("cache", ck);
+	check_distinct("cache", cv);
 	a.fill = !q_out;
 	if (q && !q_out)
 		q_out = at::empty(q->sizes(), q->options());
-	else if (q)
+	else if (q) {
 		check_like("q_out", *q_out, *q, false);
+		check_distinct("q_out", *q_out);
+	}
 	if (c.total == 0 || !k.is_cuda())
 		return q_out;
 	check_strides("k", k, 8);
@@ -270,20 +292,20 @@ Maybe append(const Tensor &ck, const Tensor &cv, const Maybe &k_scale,
 		check_strides("q", *q, 8);
 		check_strides("q_out", *q_out, 8);
 		a.q = q->data_ptr();
-		a.q_row = q->stride(0);
-		a.q_head = q->stride(1);
+		a.q_row = step(*q, 0);
+		a.q_head = step(*q, 1);
 		a.q_out = q_out->data_ptr();
-		a.q_out_row = q_out->stride(0);
-		a.q_out_head = q_out->stride(1);
+		a.q_out_row = step(*q_out, 0);
+		a.q_out_head = step(*q_out, 1);
 	}
 	if (rotation)
 		check_strides("rotation", *rotation, 4);
 	a.k = k.data_ptr();
-	a.k_row = k.stride(0);
-	a.k_head = k.stride(1);
+	a.k_row = step(k, 0);
+	a.k_head = step(k, 1);
 	a.v = v.data_ptr();
-	a.v_row = v.stride(0);
-	a.v_head = v.stride(1);
+	a.v_row = step(v, 0);
+	a.v_head = step(v, 1);
 	launched("kv_append", nvs_kv_append(&c, &a, (void *)stream));
 	return q_out;
 }
@@ -302,14 +324,18 @@ std::pair<Tensor, Maybe> attend(const Tensor &ck, const Tensor &cv,
 
 	if (c.dim != 64 && c.dim != 128 && c.dim != 256)
 		refuse("dim ", c.dim, " is not one of 64, 128 and 256");
-	forward_only({ &q, out ? &*out : nullptr });
+	forward_only({ &ck, &cv, &q, out ? &*out : nullptr });
+	if (!std::isfinite((float)scale))
+		refuse("scale ", scale, " is not finite in 32 bits");
 	nvs_kv_attend_args a = {};
 
 	a.fill = !out;
 	if (!out)
 		out = at::empty(q.sizes(), q.options());
-	else
+	else {
 		check_like("out", *out, q, false);
+		check_distinct("out", *out);
+	}
 	Maybe lse;
 
 	if (want_lse) {
@@ -322,11 +348,11 @@ std::pair<Tensor, Maybe> attend(const Tensor &ck, const Tensor &cv,
 	check_strides("q", q, 8);
 	check_strides("out", *out, 8);
 	a.q = q.data_ptr();
-	a.q_row = q.stride(0);
-	a.q_head = q.stride(1);
+	a.q_row = step(q, 0);
+	a.q_head = step(q, 1);
 	a.out = out->data_ptr();
-	a.out_row = out->stride(0);
-	a.out_head = out->stride(1);
+	a.out_row = step(*out, 0);
+	a.out_head = step(*out, 1);
 	a.scale = (float)scale;
 	a.window = (int)std::min(window, MOST);
 	a.max_new = (int)std::min(max_new, q.size(0));

@@ -428,7 +428,9 @@ int nvs_kv_attend(const nvs_kv *c, const nvs_kv_attend_args *a, void *work,
 	if ((bytes && (!work || !aligned(work, 16))) ||
 	    too_large((int64_t)p.narrow_blocks * c->kv_heads, 256) ||
 	    too_large((int64_t)p.wide_blocks * c->kv_heads * p.wide_parts,
-		      256))
+		      256) ||
+	    too_large((int64_t)c->batch * c->kv_heads * p.joined_rows, 64) ||
+	    (p.wide_parts > 1 && too_large((int64_t)c->total * c->heads, 64)))
 		return (int)hipErrorInvalidValue;
 	return BY_TYPE(launch_attend, *c, *a, p, (hipStream_t)stream);
 }

@@ -26,8 +26,8 @@ table[b, j // page_size].  An entry that is no page of the cache (-1, say)
 is allowed: what would be stored there is dropped, and what would be read
 there is not attended to.  The same holds for positions below zero, where
 lens is less than the rows, and behind the table.  Sequences may share
-pages that they only read; where two rows of a step have the same slot, one
-of them is stored.
+pages that they only read; where two rows of a step have the same slot, what
+it then holds is of either.
 
 Types.  bfloat16 or float16 rows; the cache in the rows' type, or in
 float8_e4m3fn with a float32 scale for each cached head (a value is stored
@@ -141,8 +141,6 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor,
     are in `out` (their logarithm is -inf in both)."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    elif not math.isfinite(scale):
-        raise ValueError(f"scale {scale} is not finite")
     if window is not None and window < 1:
         raise ValueError(f"window {window} is less than 1")
     if max_new is None:

@@ -17,6 +17,7 @@ for bfloat16, 2^-11 for float16, relative):
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
@@ -282,6 +283,35 @@ def test_unlike_lengths_in_one_batch(gpu):
                       heads=8, kv_heads=2, dim=128))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(12))
+def test_any_batch(gpu, seed):
+    """Whatever mixture of sequences: their tiles are dealt out evenly, and
+    long ones are divided anywhere."""
+    rng = random.Random(seed)
+    seqs = []
+    for _ in range(rng.choice((1, 3, 9, 40))):
+        new = rng.choice((0, 1, 1, 1, 2, 7, 30, 150))
+        seqs.append((new, new + rng.choice((0, 5, 300, 1500))))
+    dim = rng.choice((64, 128, 256))
+    kv_heads = rng.choice((1, 2, 3))
+    check_attend(
+        Step(gpu, seqs, heads=kv_heads * rng.choice((1, 4, 5)),
+             kv_heads=kv_heads, dim=dim, page=rng.choice((8, 16, 48, 64)),
+             cache=rng.choice((None, E4M3)), pad=rng.choice((0, 3)),
+             seed=seed),
+        window=rng.choice((None, None, 100)),
+        max_new=rng.choice((None, max(n for n, _ in seqs))))
+
+
+@pytest.mark.gpu
+def test_many_sequences(gpu):
+    seqs = [(1, 1 + 7 * b % 60) for b in range(1000)]
+    check_attend(Step(gpu, seqs, heads=2, kv_heads=1, uniform=True))
+    check_attend(Step(gpu, seqs[:333] + [(9, 40), (0, 0)], heads=2,
+                      kv_heads=1))
+
+
 # -- attend: rows that see little or nothing, bad pages ----------------
 
 
@@ -446,6 +476,17 @@ def test_out_may_be_q(device, new):
     cache, a = s.to()
     got = attend(cache, a["q"], a["table"], a["lens"], out=a["q"])
     assert got is a["q"] and torch.equal(got, want)
+
+
+def test_strides_of_one(device):
+    """What a dimension of one is strided by does not matter."""
+    s = Step(device, [(1, 30)], heads=1, kv_heads=1, page=1, uniform=True)
+    want = check_attend(s)
+    cache, a = s.to()
+    q = torch.as_strided(a["q"], (1, 1, 64), (3, 5, 1))
+    k, v = (torch.as_strided(x, x.shape, (64, 7, 9, 1)) for x in cache[:2])
+    got = attend(PagedCache(k, v), q, a["table"], a["lens"])
+    assert torch.equal(got, want)
 
 
 def test_shared_pages(device):
@@ -737,20 +778,22 @@ def test_another_stream(gpu):
 
 @pytest.mark.gpu
 def test_graphs(gpu):
-    """Two captured steps, replayed in turn with eager work between, follow
+    """Three captured steps, replayed in turn with eager work between, follow
     lens, table and rows as they then are."""
     steps = []
-    for new, context in ((1, 900), (20, 150)):
-        s = Step(gpu, [(new, context + new)] * 3, heads=8, kv_heads=2,
-                 dim=128, uniform=True, seed=new)
+    for seqs in ([(1, 901)] * 3, [(20, 170)] * 3,
+                 [(1, 700), (40, 90), (3, 333)]):
+        s = Step(gpu, seqs, heads=8, kv_heads=2, dim=128,
+                 uniform=len(set(seqs)) == 1, seed=len(seqs[0]))
         cache, a = s.to()
         rotation = rotation_table(a["table"].shape[1] * s.page, 128,
                                   device=gpu)
 
         def step(cache=cache, a=a, rotation=rotation):
             q = append(cache, a["k"], a["v"], a["table"], a["lens"],
-                       q=a["q"], rotation=rotation)
-            return attend(cache, q, a["table"], a["lens"])
+                       starts=a["starts"], q=a["q"], rotation=rotation)
+            return attend(cache, q, a["table"], a["lens"],
+                          starts=a["starts"])
 
         step()
         torch.cuda.synchronize()
@@ -842,6 +885,7 @@ def test_refusals(device):
                        q=q[..., :48].contiguous()))
     refused("window", att(window=0))
     refused("scale", att(scale=math.nan))
+    refused("scale", att(scale=1e300))
     refused("max_new", att(max_new=-1, starts=starts))
     refused("out", att(out=q[:2]))
     refused("out", att(out=q.float()))
@@ -857,6 +901,13 @@ def test_refusals(device):
     refused("rotation", app(rotation=torch.cat((rotation, rotation), 1)))
     refused("forward only", app(k=k.clone().requires_grad_()))
     refused("rotary", lambda: rotation_table(4, 20))
+    refused("out", att(out=q[:1].expand(4, -1, -1)))
+    refused("q_out", app(q=q, q_out=q[:, :1].expand(-1, 4, -1)))
+    refused("cache", app(c=PagedCache(cache.k, cache.v[:1].expand(
+        *cache.k.shape))))
+    held = PagedCache(cache.k.clone().requires_grad_(), cache.v)
+    refused("forward only", att(c=held))
+    refused("forward only", app(c=held))
     with torch.no_grad():
         attend(cache, q.clone().requires_grad_(), table, lens)
 
