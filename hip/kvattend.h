@@ -483,14 +483,13 @@ __device__ __forceinline__ void cover_padding(const nvs_kv &c,
 {
 	if (!c.starts)
 		return;
-	const int head = c.starts[0], tail = c.starts[c.batch];
+	const int64_t head = max(0, min(c.starts[0], c.total));
+	const int64_t tail = max(head, (int64_t)min(c.starts[c.batch], c.total));
 
-	for (int64_t row = who; row < c.total; row += many) {
-		if (row >= head && row < tail) {
-			/* On to this block's first row behind the last. */
-			row += (tail - row + many - 1) / many * many - many;
-			continue;
-		}
+	/* The rows before `head`, then those from `tail` on. */
+	for (int64_t n = who; n < head + c.total - tail; n += many) {
+		const int64_t row = n < head ? n : n - head + tail;
+
 		for (int i = threadIdx.x; i < c.heads * c.dim / 8;
 		     i += blockDim.x) {
 			const int h = i / (c.dim / 8), d = i % (c.dim / 8) * 8;
