@@ -686,7 +686,7 @@ void launch(const nvs_kv &c, const nvs_kv_attend_args &a, const nvs_plan &p,
 {
 	/* Wide rows of 16 bits: half the waves, as their tiles are twice as
 	 * large. */
-	constexpr int W = D * sizeof(C) > 256 ? 2 : 4;
+	constexpr int W = nvs_narrow_waves(D, sizeof(C));
 	const dim3 grid(p.narrow_blocks * c.kv_heads);
 
 	if (p.span == 16)

@@ -36,6 +36,11 @@ constexpr int nvs_narrow_tile(int dim, int size)
 
 /* The fewest tiles that are worth a block of their own. */
 constexpr int NARROW_LEAST = 4, WIDE_LEAST = 16;
+constexpr int nvs_narrow_waves(int dim, int size)
+{
+	return dim * size > 256 ? 2 : 4;
+}
+
 
 /* How the work of one call is divided. */
 struct nvs_plan {
@@ -43,6 +48,7 @@ struct nvs_plan {
 	int span;	 /* rows of a narrow block, 16 or 32 */
 	int joined_rows; /* rows of a sequence that may be divided there */
 	int narrow_blocks; /* narrow blocks for one cached head */
+	int narrow_whole;  /* each of them has one sequence, undivided */
 	int wide_blocks;   /* blocks of rows, for one cached head */
 	int wide_parts;	   /* wide blocks that may divide one's keys */
 	int cover; /* the launch that sees to rows of no sequence: 1 narrow,
@@ -164,6 +170,19 @@ __device__ __forceinline__ share share_of(const nvs_kv &c,
 					  int block, bool leave)
 {
 	const int lane = threadIdx.x & 63;
+
+	if (p.narrow_whole) {
+		share m = {};
+
+		if (block < c.batch) {
+			const sequence s = sequence_of(c, block);
+
+			m.b = block;
+			m.to = uniform64(narrow_tiles(
+				c, p, s, narrow_keys(c, a, p, s, tile)));
+		}
+		return m;
+	}
 	/* The tiles of sequence b0 + lane, and with those of the 63 before
 	 * it: all the card's memory has fewer than 32 bits of them. */
 	auto scan = [&](int b0, unsigned &own) {

@@ -311,6 +311,20 @@ nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, void *work,
 		p.narrow_blocks = (int)(most < want ? most :
 					want > 1   ? want :
 						     1);
+		/* Short sequences go to a block each, and no join is wanted:
+		 * with two tiles to a wave always (one token over 200 keys:
+		 * 9.2 us, 12.1 divided), with four where there are enough to
+		 * fill the card (64 over 500: 28.8, 32.5 divided; one: 13.7,
+		 * 10.9 divided). */
+		const int64_t turns =
+			ceil_div(ceil_div(keys, tile),
+				 nvs_narrow_waves(c.dim, size));
+
+		if (turns <= 2 ||
+		    (turns <= 4 && (int64_t)c.batch * c.kv_heads >= 256)) {
+			p.narrow_blocks = c.batch;
+			p.narrow_whole = 1;
+		}
 	}
 	if (most_rows > 32) {
 		p.wide_blocks =
@@ -335,7 +349,7 @@ nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, void *work,
 		p.cover = p.narrow_rows ? 1 : 2;
 
 	/* The parts' results, narrow before wide. */
-	const int64_t narrow = p.narrow_blocks > 1 ?
+	const int64_t narrow = p.narrow_blocks > 1 && !p.narrow_whole ?
 				       (int64_t)p.narrow_blocks * 2 *
 					       c.kv_heads * p.span :
 				       0;
@@ -365,7 +379,7 @@ int launch_attend(const nvs_kv &c, const nvs_kv_attend_args &a,
 		e = nvs_narrow<T, C>(c, a, p, s);
 	if (e == hipSuccess && p.wide_blocks)
 		e = nvs_wide<T, C>(c, a, p, s);
-	if (e == hipSuccess && p.narrow_blocks > 1)
+	if (e == hipSuccess && p.narrow_blocks > 1 && !p.narrow_whole)
 		e = nvs_join<T>(c, a, p, true, s);
 	if (e == hipSuccess && p.wide_parts > 1)
 		e = nvs_join<T>(c, a, p, false, s);

@@ -112,9 +112,8 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor,
     as they are in `q_out`; rows without a place in the table are zero."""
     device = k.get_device()
     fill = q_out is None
-    with _on(device):
-        q_out = load().append(*cache, k, v, table, lens, starts, q, rotation,
-                              interleaved, q_out, _stream(device))
+    q_out = _run(load().append, device, *cache, k, v, table, lens, starts, q,
+                 rotation, interleaved, q_out)
     if device < 0:
         _append_plain(cache, k, v, table, lens, starts, q, rotation,
                       interleaved, q_out, fill)
@@ -132,7 +131,8 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor,
     A row at position p sees the keys at positions up to p, with `window`
     the last `window` of them.  `scale` (default dim ** -0.5) multiplies
     the scores.  `max_new`, where given, says that no sequence has more new
-    rows than that; results never depend on it.
+    rows than that; the work is divided by it, and where it does not hold
+    only the time suffers.
 
     Returns [total, heads, dim], or goes into `out`, which may be q itself;
     with `return_lse` also the logarithm of each row's sum of exponentials,
@@ -149,10 +149,8 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor,
         raise ValueError(f"max_new {max_new} is negative")
     device = q.get_device()
     fill = out is None
-    with _on(device):
-        out, lse = load().attend(*cache, q, table, lens, starts, scale,
-                                 window or 0, max_new, out, return_lse,
-                                 _stream(device))
+    out, lse = _run(load().attend, device, *cache, q, table, lens, starts,
+                    scale, window or 0, max_new, out, return_lse)
     if device < 0:
         _attend_plain(cache, q, table, lens, starts, scale, window, out, lse,
                       fill)
@@ -172,30 +170,15 @@ def load():
     return module
 
 
-def _stream(device: int) -> int:
-    """The device's current stream.  torch.cuda.current_stream() takes as
-    long as the rest of a call."""
-    return torch._C._cuda_getCurrentRawStream(device) if device >= 0 else 0
-
-
-class _on:
-    """The device made current, where it is one and is not."""
-
-    __slots__ = ("device", "before")
-
-    def __init__(self, device: int) -> None:
-        self.device = device
-
-    def __enter__(self) -> None:
-        self.before = self.device
-        if self.device >= 0:
-            self.before = torch._C._cuda_getDevice()
-            if self.before != self.device:
-                torch.cuda.set_device(self.device)
-
-    def __exit__(self, *exc) -> None:
-        if self.before != self.device:
-            torch.cuda.set_device(self.before)
+def _run(call, device: int, *args):
+    """The call on the device's current stream, with the device current."""
+    if device < 0:
+        return call(*args, 0)
+    # torch.cuda's own functions for these take as long as the call.
+    if device == torch._C._cuda_getDevice():
+        return call(*args, torch._C._cuda_getCurrentRawStream(device))
+    with torch.cuda.device(device):
+        return call(*args, torch._C._cuda_getCurrentRawStream(device))
 
 
 # -- plain forms, for tensors on the CPU -------------------------------
