@@ -19,7 +19,8 @@ one after the other: sequence b has rows starts[b] .. starts[b + 1] - 1
 (`starts` [batch + 1], int32, rising from its first entry; none and many
 rows alike), or, without `starts`, total / batch rows each.  Row i of its n
 rows has position lens[b] - n + i.  All three are read on the device when
-the kernels run, so a captured graph follows what they then hold.
+the kernels run, so a captured graph follows what they then hold; nothing
+may change them meanwhile.
 
 Pages.  Position j of a sequence is in slot j % page_size of page
 table[b, j // page_size].  An entry that is no page of the cache (-1, say)
