@@ -208,14 +208,20 @@ nvs_kv describe(const Tensor &ck, const Tensor &cv, const Maybe &k_scale,
 	return c;
 }
 
-void forward_only(std::initializer_list<const Tensor *> tensors)
+void forward_only(std::initializer_list<const Tensor *> tensors,
+		  std::initializer_list<const Maybe *> optional)
 {
 	if (!at::GradMode::is_enabled())
 		return;
+	bool wanted = false;
+
 	for (const Tensor *t : tensors)
-		if (t && t->requires_grad())
-			refuse("forward only: call under torch.no_grad(), or "
-			       "detach the arguments");
+		wanted |= t->requires_grad();
+	for (const Maybe *t : optional)
+		wanted |= *t && (*t)->requires_grad();
+	if (wanted)
+		refuse("forward only: call under torch.no_grad(), or "
+		       "detach the arguments");
 }
 
 void launched(const char *what, int error)
@@ -273,8 +279,8 @@ Maybe append(const Tensor &ck, const Tensor &cv, const Maybe &k_scale,
 		a.rotary = (int)rotary;
 		a.interleaved = interleaved;
 	}
-	forward_only({ &ck, &cv, &k, &v, q ? &*q : nullptr,
-		       q_out ? &*q_out : nullptr });
+	forward_only({ &ck, &cv, &k, &v },
+		     { &k_scale, &v_scale, &q, &rotation, &q_out });
 	check_distinct("cache", ck);
 	check_distinct("cache", cv);
 	a.fill = !q_out;
@@ -324,7 +330,7 @@ std::pair<Tensor, Maybe> attend(const Tensor &ck, const Tensor &cv,
 
 	if (c.dim != 64 && c.dim != 128 && c.dim != 256)
 		refuse("dim ", c.dim, " is not one of 64, 128 and 256");
-	forward_only({ &ck, &cv, &q, out ? &*out : nullptr });
+	forward_only({ &ck, &cv, &q }, { &k_scale, &v_scale, &out });
 	if (!std::isfinite((float)scale))
 		refuse("scale ", scale, " is not finite in 32 bits");
 	nvs_kv_attend_args a = {};

@@ -912,6 +912,28 @@ def test_refusals(device):
         attend(cache, q.clone().requires_grad_(), table, lens)
 
 
+def test_scales_and_rotation_that_learn_are_refused(device):
+    s = Step(device, [(2, 30)], uniform=True, cache=E4M3)
+    cache, a = s.to()
+    q, k, v, table, lens = (a[n] for n in ("q", "k", "v", "table", "lens"))
+    rotation = rotation_table(table.shape[1] * cache.k.shape[1], 16,
+                              device=device)
+    for name in ("k_scale", "v_scale"):
+        held = cache._replace(
+            **{name: getattr(cache, name).clone().requires_grad_()})
+        with pytest.raises(ValueError, match="forward only"):
+            append(held, k, v, table, lens)
+        with pytest.raises(ValueError, match="forward only"):
+            attend(held, q, table, lens)
+        with torch.no_grad():
+            attend(held, q, table, lens)
+    with pytest.raises(ValueError, match="forward only"):
+        append(cache, k, v, table, lens, q=q,
+               rotation=rotation.requires_grad_())
+    with torch.no_grad():
+        append(cache, k, v, table, lens, q=q, rotation=rotation)
+
+
 @pytest.mark.gpu
 def test_refusals_of_layouts(gpu):
     s = Step(gpu, [(2, 30)], uniform=True)
