@@ -74,6 +74,9 @@ def run_sessions(args: argparse.Namespace) -> None:
     from nvshare_amd.workloads.common import die
     from nvshare_amd.workloads.session import Sessions
 
+    for name in ("batch", "bursts", "prompt", "layers", "page"):
+        if getattr(args, name) < 1:
+            die(f"session: --{name} {getattr(args, name)} is less than 1")
     turn = args.prompt + args.infers_per_burst
     model = Sessions(args.batch, args.bursts * turn, args.layers, args.heads,
                      args.kv_heads, args.head_dim, args.page, args.cache,

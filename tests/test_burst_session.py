@@ -78,3 +78,12 @@ def test_session_gpu(cache, dtype):
     res = run("--batch", "4", "--bursts", "2", "--infers-per-burst", "10",
               "--prompt", "300", "--cache", cache, "--dtype", dtype)
     assert res["infers"] == 22 and res["tokens"] == 4 * 2 * 310
+
+
+@pytest.mark.parametrize("name", ["batch", "bursts", "prompt", "layers",
+                                  "page"])
+def test_session_refuses_sizes_below_one(name, capsys):
+    with pytest.raises(SystemExit):
+        infer_burst.main(["--model", "session", "--device", "cpu",
+                          f"--{name}", "0"])
+    assert f"--{name} 0" in capsys.readouterr().err
