@@ -653,8 +653,12 @@ __global__ __launch_bounds__(256) void join_kernel(nvs_kv c,
 
 			y[i] = part_sum[place];
 			v[i] = *(const vec *)(part_out + place * D);
-			if (n >= parts)
-				y[i][0] = -INFINITY;
+			/* Beyond the parts: nothing, and not a part with
+			 * weight 0, which makes NaN of its infinities. */
+			if (n >= parts) {
+				y[i] = f32x2{ -INFINITY, 0.f };
+				v[i] = vec{};
+			}
 		}
 #pragma unroll
 		for (int i = 0; i < MANY; i++)
@@ -667,7 +671,8 @@ __global__ __launch_bounds__(256) void join_kernel(nvs_kv c,
 		for (int i = 0; i < MANY; i++) {
 			const float m = weigh(y[i][0], top);
 
-			/* A part that saw no key has weight 0 and zeros. */
+			/* A part that saw no key has weight 0 and zeros, one
+			 * whose scores are NaN weight 0 and NaN. */
 			sum += m * y[i][1];
 			x += m * v[i];
 		}

@@ -413,6 +413,36 @@ def test_infinite_value_reaches_the_rows_that_see_it(device, new):
     assert out[..., rest].isfinite().all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,length", [(1, 1301), (1, 5003), (8, 5003),
+                                        (40, 5203), (40, 17403)])
+def test_infinite_value_in_divided_keys(gpu, new, length):
+    """The same where the keys are divided and the parts joined, in the
+    first part and in the last: by a wave a row (1301 and 5203 keys) and by
+    four, none of them with a number of parts that fills their turns."""
+    s = Step(gpu, [(new, length)], heads=4, kv_heads=1, dim=128, page=64,
+             uniform=True, seed=new)
+    cache, a = s.to()
+    clean = attend(cache, a["q"], a["table"], a["lens"])
+    places = [s.slot(0, j) for j in (3, length - new)]
+    for value in (math.inf, -math.inf, math.nan):
+        for at in places:
+            cache, a = s.to()
+            cache.v[at][:, 5] = value
+            out = attend(cache, a["q"], a["table"], a["lens"])
+            want = torch.full_like(out[..., 5], value)
+            assert torch.equal(out[..., 5].nan_to_num(), want.nan_to_num())
+            assert torch.equal(out[..., 5].isnan(), want.isnan())
+            out[..., 5] = clean[..., 5]
+            assert torch.equal(out, clean)
+            # A key that is no number: nor is any row's result.
+            cache, a = s.to()
+            cache.k[at][:, 5] = math.nan
+            out, lse = attend(cache, a["q"], a["table"], a["lens"],
+                              return_lse=True)
+            assert out.isnan().all() and lse.isnan().all()
+
+
 def test_large_scores(device):
     """Scores far apart: exponentials neither overflow nor all vanish."""
     s = Step(device, [(2, 130)], dtype=torch.float16, seed=6)
