@@ -208,20 +208,28 @@ nvs_kv describe(const Tensor &ck, const Tensor &cv, const Maybe &k_scale,
 	return c;
 }
 
+/* Whether a derivative is wanted of a call with `t`: backwards, or
+ * forwards (a dual tensor, a transform's), which no_grad leaves on. */
+bool differentiated(const Tensor &t)
+{
+	if (at::GradMode::is_enabled() && t.requires_grad())
+		return true;
+	return c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+	       t._fw_grad(0).defined();
+}
+
 void forward_only(std::initializer_list<const Tensor *> tensors,
 		  std::initializer_list<const Maybe *> optional)
 {
-	if (!at::GradMode::is_enabled())
-		return;
 	bool wanted = false;
 
 	for (const Tensor *t : tensors)
-		wanted |= t->requires_grad();
+		wanted |= differentiated(*t);
 	for (const Maybe *t : optional)
-		wanted |= *t && (*t)->requires_grad();
+		wanted |= *t && differentiated(**t);
 	if (wanted)
-		refuse("forward only: call under torch.no_grad(), or "
-		       "detach the arguments");
+		refuse("forward only: detach the arguments, or, where none "
+		       "is a dual tensor, call under torch.no_grad()");
 }
 
 void launched(const char *what, int error)

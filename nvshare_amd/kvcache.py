@@ -39,8 +39,8 @@ head's values are contiguous and begin at 16 bytes.
 
 Launches go to the current stream of the tensors' device, and their
 workspace comes from torch's allocator, so both may be captured.  Forward
-only: a call that would have to be differentiated is refused.  Tensors on
-the CPU are computed with plain torch operations.  A refused argument
+only: a call that would have to be differentiated, backwards or forwards,
+is refused.  Tensors on the CPU are computed with plain torch operations.  A refused argument
 raises ValueError before anything runs; a failed launch, RuntimeError.
 """
 

@@ -21,6 +21,7 @@ import random
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from nvshare_amd.kvcache import PagedCache, append, attend, rotation_table
 from nvshare_amd.paths import ensure_kernels
@@ -962,6 +963,43 @@ def test_scales_and_rotation_that_learn_are_refused(device):
                rotation=rotation.requires_grad_())
     with torch.no_grad():
         append(cache, k, v, table, lens, q=q, rotation=rotation)
+
+
+@pytest.mark.parametrize("where", ["q", "k", "v", "k_cache", "v_cache",
+                                   "k_scale", "v_scale", "rotation", "out"])
+def test_forward_derivatives_are_refused(device, where):
+    """A tangent would be lost, and read as a derivative of zero."""
+    s = Step(device, [(2, 30)], uniform=True, cache=E4M3)
+    cache, a = s.to()
+    given = dict(zip(("k_cache", "v_cache", "k_scale", "v_scale"), cache),
+                 q=a["q"], k=a["k"], v=a["v"], out=torch.empty_like(a["q"]),
+                 rotation=rotation_table(32, 64, device=device))
+
+    def calls(g):
+        c = PagedCache(*(g[n] for n in ("k_cache", "v_cache", "k_scale",
+                                        "v_scale")))
+        return (lambda: attend(c, g["q"], a["table"], a["lens"],
+                               out=g["out"]),
+                lambda: append(c, g["k"], g["v"], a["table"], a["lens"],
+                               q=g["q"], q_out=g["out"],
+                               rotation=g["rotation"]))
+
+    tangent = torch.ones(given[where].shape, device=device).to(
+        given[where].dtype)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(given[where], tangent)
+        for n, call in enumerate(calls({**given, where: dual})):
+            if n == 0 and where in ("k", "v", "rotation"):
+                continue  # attend has none
+            refused("forward only", call)
+            with torch.no_grad():  # leaves forward derivatives on
+                refused("forward only", call)
+            with torch.inference_mode():
+                call()
+    if where == "q":
+        refused("forward only", lambda: torch.func.jvp(
+            lambda q: attend(cache, q, a["table"], a["lens"]), (a["q"],),
+            (tangent,)))
 
 
 @pytest.mark.gpu
