@@ -232,6 +232,14 @@ void forward_only(std::initializer_list<const Tensor *> tensors,
 		       "is a dual tensor, call under torch.no_grad()");
 }
 
+/* A kernel writes to `t`: autograd has to see that what it may have saved
+ * of it is gone.  (Tensors on the CPU are written to by torch.) */
+void written(const Tensor &t)
+{
+	if (!t.is_inference())
+		t.unsafeGetTensorImpl()->bump_version();
+}
+
 void launched(const char *what, int error)
 {
 	if (error)
@@ -320,6 +328,10 @@ Maybe append(const Tensor &ck, const Tensor &cv, const Maybe &k_scale,
 	a.v = v.data_ptr();
 	a.v_row = step(v, 0);
 	a.v_head = step(v, 1);
+	written(ck);
+	written(cv);
+	if (q)
+		written(*q_out);
 	launched("kv_append", nvs_kv_append(&c, &a, (void *)stream));
 	return q_out;
 }
@@ -378,6 +390,7 @@ std::pair<Tensor, Maybe> attend(const Tensor &ck, const Tensor &cv,
 
 	if (bytes)
 		work = at::empty({ bytes }, q.options().dtype(at::kByte));
+	written(*out);
 	launched("kv_attend",
 		 nvs_kv_attend(&c, &a, bytes ? work.data_ptr() : nullptr,
 			       (void *)stream));

@@ -1002,6 +1002,36 @@ def test_forward_derivatives_are_refused(device, where):
             (tangent,)))
 
 
+@pytest.mark.parametrize("where", ["k_cache", "v_cache", "q_out", "out"])
+def test_autograd_sees_what_is_written(device, where):
+    """What a backward pass has saved and a call overwrites is refused
+    there."""
+    s = Step(device, [(2, 30)], uniform=True)
+    cache, a = s.to()
+    mine = torch.empty_like(a["q"])
+    saved = {"k_cache": cache.k, "v_cache": cache.v}.get(where, mine)
+
+    def run():
+        factor = torch.ones((), dtype=s.q.dtype, device=device,
+                            requires_grad=True)
+        y = (factor * saved).sum()
+        if where == "out":
+            attend(cache, a["q"], a["table"], a["lens"], out=mine)
+        else:
+            append(cache, a["k"], a["v"], a["table"], a["lens"], q=a["q"],
+                   q_out=mine)
+        return y
+
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        run().backward()
+    with torch.inference_mode():  # where versions are not kept
+        mine = mine.clone()
+        cache = PagedCache(*(x.clone() for x in cache[:2]))
+        append(cache, a["k"], a["v"], a["table"], a["lens"], q=a["q"],
+               q_out=mine)
+        attend(cache, a["q"], a["table"], a["lens"], out=mine)
+
+
 @pytest.mark.gpu
 def test_refusals_of_layouts(gpu):
     s = Step(gpu, [(2, 30)], uniform=True)
