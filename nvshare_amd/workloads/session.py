@@ -65,6 +65,12 @@ class Sessions(nn.Module):
                                                device=self.device)
         self.width, self.batch, self.tokens = heads * dim, batch, 0
         self.answer = None
+        # What a word of a row, and a row of a session, count for.
+        g = torch.Generator().manual_seed(0)
+        words = kv_heads * dim * held.itemsize // 4
+        self.place, self.position = (
+            torch.randint(-2**62, 2**62, n, generator=g).mul_(2).add_(1).to(
+                self.device) for n in ((words,), (batch, per_seq * page)))
 
     @torch.no_grad()
     def step(self, new: int) -> torch.Tensor:
@@ -79,18 +85,26 @@ class Sessions(nn.Module):
         return x
 
     def fingerprint(self) -> list[int]:
-        """Sums over all that the sessions have stored, bit for bit."""
+        """A sum over all that the sessions have stored, for each cache, in
+        which a word counts by the session, position and place in the row
+        that it is at: odd random factors, so that a changed bit always
+        shows, and exchanged rows or pages do."""
         page = self.caches[0].k.shape[1]
-        used = self.table[:, :-(-self.tokens // page)].long().flatten()
         got = []
         for cache in self.caches:
             for x in (cache.k, cache.v):
-                bits = x.view(torch.uint8)[used].view(torch.int32)
-                if self.tokens % page:
-                    # The last page's unwritten slots hold anything.
-                    bits = bits.view(self.batch, -1, page, bits[0, 0].numel())
-                    bits = bits.flatten(1, 2)[:, :self.tokens]
-                got.append(int(bits.sum(dtype=torch.int64)))
+                total = torch.zeros((), dtype=torch.int64,
+                                    device=self.device)
+                for b in range(self.batch):
+                    for at in range(0, self.tokens, 64 * page):
+                        # The last page's unwritten slots hold anything.
+                        end = min(at + 64 * page, self.tokens)
+                        used = self.table[b, at // page:-(-end // page)]
+                        bits = x.view(torch.uint8)[used.long()]
+                        bits = bits.flatten(2).view(torch.int32).flatten(0, 1)
+                        rows = (bits[:end - at] * self.place).sum(-1)
+                        total += (rows * self.position[b, at:end]).sum()
+                got.append(int(total))
         return got
 
     def check(self) -> float:

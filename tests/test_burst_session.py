@@ -52,6 +52,26 @@ def test_session_notices_a_changed_cache(cache):
     assert m.fingerprint() != before
 
 
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_session_notices_exchanged_places(cache):
+    """Pages of two sessions, pages of one, rows, and words exchanged."""
+    m = Sessions(2, 40, layers=1, heads=2, kv_heads=1, dim=64, page=16,
+                 cache=cache, device="cpu")
+    m.step(35)
+    before = m.fingerprint()
+    k = m.caches[0].k.view(torch.uint8)
+    (a, b), c = m.table[:, 0].tolist(), int(m.table[0, 1])
+    for one, other in (((a,), (b,)), ((a,), (c,)), ((a, 3), (a, 9)),
+                       ((a, 3, 0, slice(0, 4)), (a, 3, 0, slice(8, 12)))):
+        held = k.clone()
+        k[one], k[other] = held[other], held[one]
+        assert m.fingerprint() != before
+        k.copy_(held)
+        assert m.fingerprint() == before
+    m.caches[0] = m.caches[0]._replace(k=m.caches[0].v, v=m.caches[0].k)
+    assert m.fingerprint() != before
+
+
 def test_session_notices_a_wrong_answer():
     m = Sessions(1, 40, layers=1, heads=2, kv_heads=1, dim=64, page=16,
                  device="cpu")
