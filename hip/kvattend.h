@@ -502,8 +502,17 @@ __device__ __forceinline__ void cover_padding(const nvs_kv &c,
 {
 	if (!c.starts)
 		return;
-	const int64_t head = max(0, min(c.starts[0], c.total));
-	const int64_t tail = max(head, (int64_t)min(c.starts[c.batch], c.total));
+	const int *starts = c.starts;
+	const int64_t head = max(0, min(starts[0], c.total));
+	/* Sequences that pass the rows have none of them. */
+	int64_t tail = starts[c.batch];
+
+	if (tail > c.total)
+		tail = starts[last_at_most(
+			c.batch, c.total, [=](int i) {
+				return (int64_t)starts[i];
+			})];
+	tail = max(head, min(tail, (int64_t)c.total));
 
 	/* The rows before `head`, then those from `tail` on. */
 	for (int64_t n = who; n < head + c.total - tail; n += many) {

@@ -105,13 +105,16 @@ __global__ __launch_bounds__(256) void append_kernel(nvs_kv c,
 	if (row64 >= c.total)
 		return;
 	const int row = (int)row64;
-	const int b = sequence_at(c, row);
+	int b = sequence_at(c, row);
 	int64_t pos = -1;
 
 	if (b >= 0) {
 		const sequence s = sequence_of(c, b);
 
-		pos = s.pos + (row - s.first);
+		if (row - s.first < s.count)
+			pos = s.pos + (row - s.first);
+		else
+			b = -1;
 	}
 	const int capacity = c.per_seq * c.page_size;
 	const bool in_range = pos >= 0 && pos < capacity;

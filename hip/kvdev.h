@@ -122,7 +122,8 @@ __device__ __forceinline__ sequence sequence_of(const nvs_kv &c, int b)
 	if (c.starts) {
 		s.first = c.starts[b];
 		s.count = c.starts[b + 1] - s.first;
-		/* Never beyond the rows, whatever starts holds. */
+		/* Never beyond the rows, whatever starts holds: a sequence
+		 * that would be has none of them. */
 		if (s.first < 0 || s.count < 0 || s.first > c.total ||
 		    s.count > c.total - s.first)
 			s.count = 0;

@@ -17,8 +17,9 @@ order, `lens` [batch] (int32) the tokens that it has, those of this step
 included.  The step's rows q, k, v [total, heads, dim] hold the sequences
 one after the other: sequence b has rows starts[b] .. starts[b + 1] - 1
 (`starts` [batch + 1], int32, rising from its first entry; none and many
-rows alike), or, without `starts`, total / batch rows each.  Row i of its n
-rows has position lens[b] - n + i.  All three are read on the device when
+rows alike; a sequence whose rows would pass total has none, and the rows
+are of no sequence), or, without `starts`, total / batch rows each.  Row i
+of its n rows has position lens[b] - n + i.  All three are read on the device when
 the kernels run, so a captured graph follows what they then hold; nothing
 may change them meanwhile.
 
@@ -194,6 +195,8 @@ def _sequences(total, lens, starts):
         bounds = starts.tolist()
     for b, length in enumerate(lens.tolist()):
         lo, hi = bounds[b], bounds[b + 1]
+        if not 0 <= lo <= hi <= total:
+            lo = hi = 0
         yield b, slice(lo, hi), torch.arange(length - (hi - lo), length)
 
 

@@ -665,6 +665,34 @@ def test_append_padding_rows(device):
     assert (mine[4:] == 7.0).all() and torch.equal(mine[:4], q[:4])
 
 
+@pytest.mark.parametrize("bounds", [[0, 3, 4, 99], [0, 3, 9, 99],
+                                    [5, 90, 95, 99], [0, 3, 5, 2**31 - 1],
+                                    [99, 99, 99, 99]])
+@pytest.mark.parametrize("max_new", [None, 2])
+def test_sequences_that_pass_the_rows_have_none(device, bounds, max_new):
+    """Neither operator takes their rows for a token: they are padding."""
+    s = Step(device, [(3, 40), (1, 70), (2, 30)], seed=9)
+    total = s.q.shape[0]
+    s.bounds, s.starts = bounds, torch.tensor(bounds, dtype=torch.int32)
+    s.seqs = [(hi - lo if hi <= total else 0, t) for (lo, hi), (_, t) in zip(
+        zip(bounds, bounds[1:]), s.seqs)]
+    used = sorted(row for row, _, _ in s.rows())
+    free = [row for row in range(total) if row not in used]
+    assert free
+    q, _ = check_append(s)
+    out = check_attend(s, max_new=max_new)
+    assert not q[free].any() and not out[free].any()
+    cache, a = s.to()
+    for call in (lambda mine: append(
+            cache, a["k"], a["v"], a["table"], a["lens"],
+            starts=a["starts"], q=a["q"], q_out=mine),
+            lambda mine: attend(cache, a["q"], a["table"], a["lens"],
+                                starts=a["starts"], out=mine)):
+        mine = torch.full_like(a["q"], 7.0)
+        call(mine)
+        assert (mine[free] == 7.0).all()
+
+
 def test_append_in_place_and_strided(device):
     s = Step(device, [(9, 40), (2, 70)], heads=6, kv_heads=2, dim=128)
     q, cache = check_append(s)
