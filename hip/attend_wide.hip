@@ -468,6 +468,14 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 					out[d] *= keep;
 			}
 			const float unit = sm.unit(f.c);
+			/* Weights are rounded once to T before they meet the
+			 * values; their sum is made of the unrounded ones.
+			 * With the results' own rounding that is 2.4e-3 of
+			 * their size in bfloat16, 2.9e-4 in float16, where
+			 * two parts of T, as the narrow kernel has, leave
+			 * 1.7e-3 and 2.1e-4 and half as many products again:
+			 * 1385 us instead of 1054 (the chunk above), 484
+			 * instead of 394 (ragged prompts of up to 4096). */
 			u32x4 weight[4];
 #pragma unroll
 			for (int h = 0; h < 2; h++) {

@@ -69,6 +69,42 @@ __device__ __forceinline__ unsigned pack2(float a, float b)
 	return __builtin_bit_cast(unsigned, v);
 }
 
+/* Two weights (0 or more), each as a number cut off after T's bits and the
+ * rest of it, rounded to nearest: {both first parts, both rests}.  The rest
+ * of a weight that is not 0 is not 0 either (what is added is at most 2^-20
+ * of the weight, or T's smallest number), and no part is negative, so that
+ * infinity times both is infinity. */
+template <typename T>
+__device__ __forceinline__ u32x2 split2(float a, float b)
+{
+	constexpr float MORE = 1.f + 0x1p-20f;
+
+	if constexpr (__is_same(T, bf16_t)) {
+		const unsigned u = __builtin_bit_cast(unsigned, a);
+		const unsigned v = __builtin_bit_cast(unsigned, b);
+		const float ha = __builtin_bit_cast(float, u & 0xffff0000u);
+		const float hb = __builtin_bit_cast(float, v & 0xffff0000u);
+
+		return u32x2{ u >> 16 | (v & 0xffff0000u),
+			      pack2<T>(__builtin_fmaf(a, MORE, -ha),
+				       __builtin_fmaf(b, MORE, -hb)) };
+	} else {
+		typedef unsigned short u16x2
+			__attribute__((ext_vector_type(2)));
+		const fp16x2 h = __builtin_bit_cast(
+			fp16x2, __builtin_amdgcn_cvt_pkrtz(a, b));
+		const u16x2 n = __builtin_bit_cast(u16x2, h);
+
+		const unsigned rest =
+			pack2<T>(__builtin_fmaf(a, MORE, -(float)h[0]),
+				 __builtin_fmaf(b, MORE, -(float)h[1]));
+		const u16x2 least = __builtin_elementwise_min(n, u16x2{ 1, 1 });
+
+		return u32x2{ __builtin_bit_cast(unsigned, h),
+			      rest | __builtin_bit_cast(unsigned, least) };
+	}
+}
+
 /* Two e4m3 numbers as T: exact in both types. */
 template <typename T, bool HIGH>
 __device__ __forceinline__ unsigned widen2(unsigned w)

@@ -463,6 +463,67 @@ def test_scores_rise_along_the_keys(device, new):
     check_attend(s)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cache", [None, E4M3])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 6, 14])
+def test_weights_of_few_rows_keep_their_bits(device, dtype, cache, dim, new):
+    """Up to 32 rows of a sequence: weights meet the values in two parts.
+    With u half a step, the first part (cut off) leaves 2u, and that is
+    rounded to u: 2u^2; two additions that keep parts from being zero are
+    2^-20 each, or 2^-24 of 2^11 for each key in float16.  Small queries
+    leave next to nothing to the scores' own errors."""
+    s = Step(device, [(new, 20)], dtype=dtype, cache=cache, dim=dim,
+             uniform=True, seed=dim + new)
+    s.q /= 16
+    u = half_step(dtype)
+    cache, a = s.to("cpu")
+    k, v = (torch.stack([x[s.slot(0, j)] for j in range(20)]).double()
+            for x in cache[:2])
+    if s.cache.k_scale is not None:
+        k, v = (x * c.double()[:, None] for x, c in zip((k, v), cache[2:]))
+    k, v = (x.repeat_interleave(2, 1).transpose(0, 1) for x in (k, v))
+    q = s.q.double().transpose(0, 1)
+    scale = dim**-0.5
+    hidden = torch.arange(20) > torch.arange(20 - new, 20)[:, None]
+    w = (q @ k.transpose(1, 2) * scale).masked_fill(hidden, -math.inf)
+    w = w.softmax(-1)
+    want, size = w @ v, w @ v.abs()
+    off = dim * 2.0**-24 * scale * (q.abs() @ k.abs().transpose(1, 2)).max()
+    tol = u * want.abs() + (2 * u * u + 2.0**-19 + 2 * off + 2.0**-20) * size
+    if dtype == torch.float16:
+        tol += 20 * 2.0**-35 * size.max() + 2.0**-25
+    cache, a = s.to()
+    got = attend(cache, a["q"], a["table"], a["lens"])
+    near(got, want.transpose(0, 1), 1.01 * tol.transpose(0, 1), "out")
+
+
+@pytest.mark.parametrize("new", [1, 6])
+@pytest.mark.parametrize("dtype,less", [(torch.bfloat16, 1e-3),
+                                        (torch.bfloat16, 60.0),
+                                        (torch.float16, 1e-3),
+                                        (torch.float16, 15.0)])
+def test_infinite_values_with_little_weight(device, new, dtype, less):
+    """They reach the rows that see them whatever a weight leaves behind
+    its first bits: nothing at all where it is a power of two."""
+    s = Step(device, [(new, 100)], dtype=dtype, uniform=True)
+    s.q.zero_()
+    s.cache.k.zero_()
+    s.q[..., 0] = 8.0
+    for j in (11, 70):
+        at = s.slot(0, j)
+        s.cache.k[at][:, 0] = -less
+        s.cache.v[at][:, 5] = math.inf
+        s.cache.v[at][:, 6] = -math.inf
+    at = s.slot(0, 40)  # as much weight as the others: a power of two
+    s.cache.v[at][:, 7] = math.inf
+    cache, a = s.to()
+    out = attend(cache, a["q"], a["table"], a["lens"])
+    assert (out[..., 5] == math.inf).all() and (
+        out[..., 6] == -math.inf).all() and (out[..., 7] == math.inf).all()
+    assert out[..., 8:].isfinite().all()
+
+
 # -- attend: buffers ---------------------------------------------------
 
 
