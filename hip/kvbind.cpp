@@ -9,6 +9,8 @@
  */
 #include <torch/extension.h>
 
+#include <dlfcn.h>
+
 #include <cmath>
 #include <limits>
 #include <optional>
@@ -16,17 +18,47 @@
 
 #include "kvcache.h"
 
-extern "C" {
-int nvs_kv_append(const nvs_kv *c, const nvs_kv_append_args *a, void *stream);
-int64_t nvs_kv_attend_work(const nvs_kv *c, const nvs_kv_attend_args *a);
-int nvs_kv_attend(const nvs_kv *c, const nvs_kv_attend_args *a, void *work,
-		  void *stream);
-}
-
 namespace {
 
 using at::Tensor;
 using Maybe = std::optional<Tensor>;
+
+/* The kernels' library, which lies beside this one.  It is loaded for the
+ * first launch only: tensors on the CPU need neither it nor a GPU's runtime.
+ */
+struct entries {
+	int (*append)(const nvs_kv *c, const nvs_kv_append_args *a,
+		      void *stream);
+	int64_t (*attend_work)(const nvs_kv *c, const nvs_kv_attend_args *a);
+	int (*attend)(const nvs_kv *c, const nvs_kv_attend_args *a, void *work,
+		      void *stream);
+};
+
+const entries &kernels()
+{
+	static const entries e = [] {
+		void *lib = dlopen("libnvshare_hiputil.so",
+				   RTLD_NOW | RTLD_LOCAL);
+		auto entry = [&](const char *name) {
+			void *p = lib ? dlsym(lib, name) : nullptr;
+
+			if (!p)
+				throw std::runtime_error(
+					std::string(dlerror()) +
+					"; build with `make -C hip` (hipcc, "
+					"gfx950)");
+			return p;
+		};
+		entries got;
+
+		got.append = (decltype(got.append))entry("nvs_kv_append");
+		got.attend_work = (decltype(got.attend_work))entry(
+			"nvs_kv_attend_work");
+		got.attend = (decltype(got.attend))entry("nvs_kv_attend");
+		return got;
+	}();
+	return e;
+}
 
 constexpr int64_t MOST = std::numeric_limits<int32_t>::max();
 
@@ -332,7 +364,7 @@ Maybe append(const Tensor &ck, const Tensor &cv, const Maybe &k_scale,
 	written(cv);
 	if (q)
 		written(*q_out);
-	launched("kv_append", nvs_kv_append(&c, &a, (void *)stream));
+	launched("kv_append", kernels().append(&c, &a, (void *)stream));
 	return q_out;
 }
 
@@ -382,7 +414,7 @@ std::pair<Tensor, Maybe> attend(const Tensor &ck, const Tensor &cv,
 	a.scale = (float)scale;
 	a.window = (int)std::min(window, MOST);
 	a.max_new = (int)std::min(max_new, q.size(0));
-	const int64_t bytes = nvs_kv_attend_work(&c, &a);
+	const int64_t bytes = kernels().attend_work(&c, &a);
 
 	if (bytes < 0)
 		launched("kv_attend", 1);
@@ -392,8 +424,8 @@ std::pair<Tensor, Maybe> attend(const Tensor &ck, const Tensor &cv,
 		work = at::empty({ bytes }, q.options().dtype(at::kByte));
 	written(*out);
 	launched("kv_attend",
-		 nvs_kv_attend(&c, &a, bytes ? work.data_ptr() : nullptr,
-			       (void *)stream));
+		 kernels().attend(&c, &a, bytes ? work.data_ptr() : nullptr,
+				  (void *)stream));
 	return { *out, lse };
 }
 

@@ -41,8 +41,10 @@ head's values are contiguous and begin at 16 bytes.
 Launches go to the current stream of the tensors' device, and their
 workspace comes from torch's allocator, so both may be captured.  Forward
 only: a call that would have to be differentiated, backwards or forwards,
-is refused.  Tensors on the CPU are computed with plain torch operations.  A refused argument
-raises ValueError before anything runs; a failed launch, RuntimeError.
+is refused.  Tensors on the CPU are computed with plain torch operations;
+they need the compiled calls (hip/kvbind.cpp, a C++ compiler's work) and
+not the kernels.  A refused argument raises ValueError before anything
+runs; a failed launch, RuntimeError.
 """
 
 from __future__ import annotations
@@ -165,7 +167,9 @@ def load():
     path = artifacts().kvbind
     if not path.exists():
         raise FileNotFoundError(
-            f"{path} missing; build with `make -C hip` (hipcc, gfx950)")
+            f"{path} missing; build with `make -C hip` (hipcc, gfx950), or "
+            "for tensors on the CPU `make -C hip build/_kvbind.so` (a C++ "
+            "compiler)")
     spec = importlib.util.spec_from_file_location("_kvbind", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)

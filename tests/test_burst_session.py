@@ -4,13 +4,14 @@ them, on the CPU and, with -m gpu, on an MI355X."""
 from __future__ import annotations
 
 import json
+import shutil
 import subprocess
 import sys
 
 import pytest
 import torch
 
-from nvshare_amd.paths import ensure_kernels
+from nvshare_amd.paths import REPO_ROOT, artifacts, ensure_kernels
 from nvshare_amd.workloads import infer_burst
 from nvshare_amd.workloads.session import Sessions
 
@@ -36,6 +37,53 @@ def test_session_cpu():
               "--heads", "4", "--kv-heads", "2", "--head-dim", "64",
               "--page", "16")
     assert res["infers"] == 8 and res["tokens"] == 2 * 2 * 12
+
+
+ALONE = """
+import pathlib, sys
+from nvshare_amd import paths
+paths.HIP_BUILD_DIR = pathlib.Path(sys.argv[1])
+"""
+
+
+def alone(tmp_path, code, *args):
+    """Runs the code where the kernels' library has not been built."""
+    shutil.copy(artifacts().kvbind, tmp_path)
+    return subprocess.run(
+        [sys.executable, "-c", ALONE + code, str(tmp_path), *args],
+        capture_output=True, text=True, timeout=240, cwd=REPO_ROOT)
+
+
+def test_session_cpu_without_kernels(tmp_path):
+    r = alone(tmp_path, """
+from nvshare_amd.workloads.infer_burst import main
+main(sys.argv[2:])
+""", "--model", "session", "--device", "cpu", "--batch", "1", "--bursts",
+              "1", "--infers-per-burst", "1", "--prompt", "3", "--layers",
+              "1", "--heads", "1", "--kv-heads", "1", "--head-dim", "64",
+              "--think-s", "0")
+    assert r.returncode == 0, r.stderr[-3000:]
+
+
+@pytest.mark.gpu
+def test_launch_without_kernels_is_an_error(tmp_path):
+    r = alone(tmp_path, """
+import torch
+from nvshare_amd import kvcache
+cache = kvcache.PagedCache.empty(2, 16, 1, 64)
+q = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda")
+one = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+for call in (lambda: kvcache.attend(cache, q, one, one[0]),
+             lambda: kvcache.append(cache, q, q, one, one[0])):
+    try:
+        call()
+    except RuntimeError as e:
+        assert "libnvshare_hiputil.so" in str(e), e
+        assert "make -C hip" in str(e), e
+    else:
+        raise SystemExit("no error")
+""")
+    assert r.returncode == 0, r.stderr[-3000:]
 
 
 @pytest.mark.parametrize("cache", ["same", "e4m3"])
