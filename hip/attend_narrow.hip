@@ -289,17 +289,23 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 		auto is_whole = [&](int pages) {
 			return one_page && __all(pages >= 0);
 		};
-		/* The table's entry for key lane % TILE of a tile, or the
-		 * nearest one that some row sees. */
+		/* Key lane % TILE of a tile; below zero where one beyond the
+		 * last passes 31 bits. */
+		auto key_of = [&](int tile) {
+			return (int)((unsigned)tile * TILE +
+				     (lane & (TILE - 1)));
+		};
+		/* The table's entry for it, or the nearest one that some row
+		 * sees. */
 		auto entry = [&](int tile) {
-			const int key = tile * TILE + (lane & (TILE - 1));
+			const int key = key_of(tile);
 
 			return table + entry_of(p, min(max(key, k.lo),
 						       k.hi - 1));
 		};
 		/* The pages, -1 for keys that no row sees. */
 		auto pages_of = [&](int tile, int entry) {
-			const int key = tile * TILE + (lane & (TILE - 1));
+			const int key = key_of(tile);
 
 			return key >= k.lo && key < k.hi && is_page(c, entry) ?
 				       entry :

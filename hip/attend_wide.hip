@@ -404,7 +404,8 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 			}
 		}
 
-		if (!idle && key0 <= most_lim && key0 + TILE > least_low) {
+		if (!idle && key0 <= most_lim &&
+		    key0 + TILE - 1 >= least_low) {
 			/* Keys: S^T = K Q^T. */
 			f32x16 score[2];
 #pragma unroll

@@ -957,6 +957,21 @@ def test_offsets_beyond_32_bits(gpu):
     near(cache.v[base:], w[4], w[5], "v")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("length", [2147483600, 2147483599, 2147483580])
+@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_last_positions_of_31_bits(gpu, length, new, dim):
+    """Tables name up to 2^31 - 1 positions; the last tile of these ends
+    beyond that."""
+    s = Step(gpu, [(new, 300)], page=100, pages=5, dim=dim)
+    s.table = (torch.arange(21474836, dtype=torch.int32) % 5)[None]
+    s.lens = torch.tensor([length], dtype=torch.int32)
+    s.seqs = [(new, length)]
+    check_attend(s, window=70)
+    check_append(s, rotary=0)
+
+
 # -- refusals ----------------------------------------------------------
 
 
