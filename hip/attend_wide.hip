@@ -404,8 +404,7 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 			}
 		}
 
-		if (!idle && key0 <= most_lim &&
-		    key0 + TILE - 1 >= least_low) {
+		if (!idle && key0 <= most_lim && key0 > least_low - TILE) {
 			/* Keys: S^T = K Q^T. */
 			f32x16 score[2];
 #pragma unroll

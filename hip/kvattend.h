@@ -95,7 +95,7 @@ __device__ __forceinline__ key_range keys_of(const nvs_kv &c, int window,
 	if (k.hi <= k.lo)
 		k.lo = k.hi = 0;
 	k.first = k.lo / tile;
-	k.last = k.hi ? (k.hi - 1) / tile + 1 : 0; /* hi may be 2^31 - 1 */
+	k.last = (int)(((unsigned)k.hi + tile - 1) / tile);
 	return k;
 }
 
