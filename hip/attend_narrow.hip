@@ -187,12 +187,11 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 					low[n] = (int)max(s.pos + i - a.window,
 							  (int64_t)-1);
 #pragma unroll
-				for (int d = 0; d < D / 32; d++) {
+				for (int d = 0; d < D / 32; d++)
 					q[n][d] = *(const u32x4 *)(src +
 								   32 * d +
 								   8 * quarter);
-					q[n][d] = (q[n][d] ^ f.flip) & f.keep;
-				}
+				factored<T>(f, q[n]);
 			} else {
 #pragma unroll
 				for (int d = 0; d < D / 32; d++)

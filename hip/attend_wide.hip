@@ -151,8 +151,8 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 		q[d] = u32x4{};
 		if (real)
 			q[d] = *(const u32x4 *)(src + 16 * d + 8 * half);
-		q[d] = (q[d] ^ f.flip) & f.keep;
 	}
+	factored<T>(f, q);
 
 	softmax<T> sm;
 	f32x16 out[D / 32];

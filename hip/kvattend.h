@@ -396,23 +396,6 @@ template <typename T> struct softmax {
 	}
 };
 
-/* The factor of a row's scores, and what its queries are multiplied by
- * (as bits: a sign to flip, or all to clear) so that it is positive: the
- * largest score then has the largest weight. */
-struct factor {
-	float c;
-	unsigned flip, keep;
-};
-
-__device__ __forceinline__ factor factor_of(float c)
-{
-	factor f = { fabsf(c), c < 0.f ? 0x80008000u : 0u, ~0u };
-
-	if (c == 0.f)
-		f = { 1.f, 0u, 0u };
-	return f;
-}
-
 /* Whether one of two numbers of type T (four e4m3) is infinite or NaN. */
 template <typename C> __device__ __forceinline__ bool not_finite(unsigned w)
 {
@@ -434,6 +417,46 @@ template <typename C> __device__ __forceinline__ unsigned finite_only(unsigned w
 		if (not_finite<C>(w & (FIELD << i)))
 			w &= ~(FIELD << i);
 	return w;
+}
+
+/* The factor of a row's scores, and what makes it positive, so that the
+ * largest score has the largest weight: a sign to flip in the queries' bits,
+ * or (zero) queries of zero. */
+struct factor {
+	float c;
+	unsigned flip;
+	bool zero;
+};
+
+__device__ __forceinline__ factor factor_of(float c)
+{
+	if (c == 0.f)
+		return { 1.f, 0u, true };
+	return { fabsf(c), c < 0.f ? 0x80008000u : 0u, false };
+}
+
+/* 0 times a word of T: NaN for what is infinite or NaN. */
+template <typename T> __device__ __forceinline__ unsigned times_zero(unsigned w)
+{
+	return (not_finite<T>(w & 0xffffu) ? 0x7fffu : 0u) |
+	       (not_finite<T>(w & 0xffff0000u) ? 0x7fff0000u : 0u);
+}
+
+/* The pieces of a row's queries, as its factor wants them. */
+template <typename T, int N>
+__device__ __forceinline__ void factored(const factor &f, u32x4 (&q)[N])
+{
+#pragma unroll
+	for (int d = 0; d < N; d++)
+		q[d] ^= f.flip;
+	if (f.zero) {
+		rarely();
+#pragma unroll
+		for (int d = 0; d < N; d++)
+#pragma unroll
+			for (int e = 0; e < 4; e++)
+				q[d][e] = times_zero<T>(q[d][e]);
+	}
 }
 
 /* x if it is infinite or NaN, else 0. */

@@ -383,6 +383,25 @@ def test_later_tokens_hold_anything(device, value, new, heads):
     assert not out[-1].isfinite().all()
 
 
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new", [1, 40])
+def test_queries_that_are_no_numbers(device, value, dtype, new):
+    """Nor is their result, whatever the scores are multiplied by: 0 too."""
+    s = Step(device, [(new, 60)], dtype=dtype, uniform=True)
+    s.q[0, 1, 3] = value
+    for scale in (None, -0.5, 0.0):
+        cache, a = s.to()
+        out, lse = attend(cache, a["q"], a["table"], a["lens"], scale=scale,
+                          return_lse=True)
+        spoilt = torch.zeros(new, 4, dtype=torch.bool, device=device)
+        spoilt[0, 1] = True
+        # Of infinite scores the sum is infinite, if not NaN.
+        assert torch.equal(~lse.isfinite(), spoilt)
+        assert torch.equal(out.isnan(), spoilt[..., None].expand_as(out))
+        assert out[~spoilt].isfinite().all()
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf])
 @pytest.mark.parametrize("new", [1, 5, 66])
 def test_tokens_before_the_window_hold_anything(device, value, new):
