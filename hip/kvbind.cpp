@@ -290,9 +290,10 @@ Maybe append(const Tensor &ck, const Tensor &cv, const Maybe &k_scale,
 {
 	check_rows("k", k);
 	check_like("v", v, k, false);
-	if (q)
+	if (q) {
+		check_rows("q", *q);
 		check_like("q", *q, k, true);
-	else if (q_out)
+	} else if (q_out)
 		refuse("q_out without q");
 	const nvs_kv c = describe(ck, cv, k_scale, v_scale, k,
 				  q ? q->size(1) : k.size(1), table, lens,
@@ -373,7 +374,9 @@ std::pair<Tensor, Maybe> attend(const Tensor &ck, const Tensor &cv,
 				const Maybe &k_scale, const Maybe &v_scale,
 				const Tensor &q, const Tensor &table,
 				const Tensor &lens, const Maybe &starts,
-				double scale, int64_t window, int64_t max_new,
+				std::optional<double> given_scale,
+				int64_t window,
+				std::optional<int64_t> max_new,
 				Maybe out, bool want_lse, uintptr_t stream)
 {
 	check_rows("q", q);
@@ -383,6 +386,8 @@ std::pair<Tensor, Maybe> attend(const Tensor &ck, const Tensor &cv,
 	if (c.dim != 64 && c.dim != 128 && c.dim != 256)
 		refuse("dim ", c.dim, " is not one of 64, 128 and 256");
 	forward_only({ &ck, &cv, &q }, { &k_scale, &v_scale, &out });
+	const double scale = given_scale.value_or(std::pow(c.dim, -0.5));
+
 	if (!std::isfinite((float)scale))
 		refuse("scale ", scale, " is not finite in 32 bits");
 	nvs_kv_attend_args a = {};
@@ -413,7 +418,7 @@ std::pair<Tensor, Maybe> attend(const Tensor &ck, const Tensor &cv,
 	a.out_head = step(*out, 1);
 	a.scale = (float)scale;
 	a.window = (int)std::min(window, MOST);
-	a.max_new = (int)std::min(max_new, q.size(0));
+	a.max_new = (int)std::min(max_new.value_or(q.size(0)), q.size(0));
 	const int64_t bytes = kernels().attend_work(&c, &a);
 
 	if (bytes < 0)

@@ -143,19 +143,17 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor,
     float32 [total, heads].  A row that sees no key gives zeros, and -inf.
     Rows of no sequence give the same in a new tensor and are left as they
     are in `out` (their logarithm is -inf in both)."""
-    if scale is None:
-        scale = q.shape[-1] ** -0.5
     if window is not None and window < 1:
         raise ValueError(f"window {window} is less than 1")
-    if max_new is None:
-        max_new = q.shape[0]
-    elif max_new < 0:
+    if max_new is not None and max_new < 0:
         raise ValueError(f"max_new {max_new} is negative")
     device = q.get_device()
     fill = out is None
     out, lse = _run(load().attend, device, *cache, q, table, lens, starts,
                     scale, window or 0, max_new, out, return_lse)
     if device < 0:
+        if scale is None:
+            scale = q.shape[-1] ** -0.5
         _attend_plain(cache, q, table, lens, starts, scale, window, out, lse,
                       fill)
     return (out, lse) if return_lse else out

@@ -1066,6 +1066,20 @@ def test_refusals(device):
         attend(cache, q.clone().requires_grad_(), table, lens)
 
 
+def test_rows_of_no_shape_are_refused(device):
+    """Before anything is made of their dimensions."""
+    s = Step(device, [(2, 30)], uniform=True)
+    cache, a = s.to()
+    k, v, table, lens = (a[n] for n in ("k", "v", "table", "lens"))
+    for q in (a["q"][0, 0, 0], a["q"][0], a["q"][..., :0]):
+        refused("", lambda: attend(cache, q, table, lens))
+        refused("q: ", lambda: append(cache, k, v, table, lens, q=q))
+    # More heads than the kernels count (and the memory of one).
+    heads = k[:, :1].expand(-1, 2**30, -1)
+    refused("31 bits", lambda: append(cache, k, v, table, lens, q=heads))
+    refused("31 bits", lambda: attend(cache, heads, table, lens))
+
+
 def test_scales_and_rotation_that_learn_are_refused(device):
     s = Step(device, [(2, 30)], uniform=True, cache=E4M3)
     cache, a = s.to()
