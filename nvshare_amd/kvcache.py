@@ -263,7 +263,10 @@ def _attend_plain(cache, q, table, lens, starts, scale, window, out, lse,
     for b, rows, pos in _sequences(q.shape[0], lens, starts):
         if not pos.numel():
             continue
-        keys = torch.arange(max(0, int(pos[-1]) + 1))
+        # From the first that some row sees to the last with a place.
+        first = max(0, int(pos[0]) + 1 - window) if window else 0
+        last = min(int(pos[-1]) + 1, table.shape[1] * cache.k.shape[1])
+        keys = torch.arange(first, max(first, last))
         _, mapped, page, slot = _slots(cache, table, b, keys)
         keys, page, slot = keys[mapped], page[mapped], slot[mapped]
         k, v = cache.k[page, slot].float(), cache.v[page, slot].float()

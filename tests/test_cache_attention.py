@@ -349,6 +349,25 @@ def test_length_behind_the_table(device):
     check_attend(s, window=9)
 
 
+@pytest.mark.parametrize("new", [1, 40])
+def test_any_length_behind_the_table(device, new):
+    """Takes no more time and memory than the table's positions."""
+    s = Step(device, [(new, 60)])
+    want = check_attend(s)
+    cache, a = s.to()
+    lens = torch.tensor([2**31 - 1], dtype=torch.int32, device=device)
+    q = a["q"][-1:].expand(new, -1, -1)
+    seen = torch.tensor([64], dtype=torch.int32, device=device)
+    last = attend(cache, a["q"][-1:], a["table"], seen)
+    out = attend(cache, q, a["table"], lens)
+    tol = 2 * half_step(s.q.dtype) * (last.abs() + s.cache.v.abs().max().to(
+        device)).double().cpu()  # rounded by other kernels
+    near(out, last.double().cpu().expand(out.shape), tol, "out")
+    assert not attend(cache, q, a["table"], lens, window=9).any()
+    assert not attend(cache, q, a["table"], lens - 2**31).any()
+    assert torch.equal(attend(cache, a["q"], a["table"], a["lens"]), want)
+
+
 def spoil(s, value, where):
     """Put `value` in every cached key and value that `where` names."""
     for b, j in where:
@@ -1072,7 +1091,7 @@ def test_rows_of_no_shape_are_refused(device):
     cache, a = s.to()
     k, v, table, lens = (a[n] for n in ("k", "v", "table", "lens"))
     for q in (a["q"][0, 0, 0], a["q"][0], a["q"][..., :0]):
-        refused("", lambda: attend(cache, q, table, lens))
+        refused("wanted|cache", lambda: attend(cache, q, table, lens))
         refused("q: ", lambda: append(cache, k, v, table, lens, q=q))
     # More heads than the kernels count (and the memory of one).
     heads = k[:, :1].expand(-1, 2**30, -1)
