@@ -74,9 +74,19 @@ def run_sessions(args: argparse.Namespace) -> None:
     from nvshare_amd.workloads.common import die
     from nvshare_amd.workloads.session import Sessions
 
-    for name in ("batch", "bursts", "prompt", "layers", "page"):
-        if getattr(args, name) < 1:
-            die(f"session: --{name} {getattr(args, name)} is less than 1")
+    for name, least in (("batch", 1), ("bursts", 1), ("prompt", 1),
+                        ("layers", 1), ("page", 1), ("heads", 1),
+                        ("kv_heads", 1), ("infers_per_burst", 0),
+                        ("think_s", 0)):
+        if not getattr(args, name) >= least:
+            die(f"session: --{name.replace('_', '-')} "
+                f"{getattr(args, name)} is less than {least}")
+    if args.heads % args.kv_heads:
+        die(f"session: --heads {args.heads} is no multiple of --kv-heads "
+            f"{args.kv_heads}")
+    if args.head_dim not in (64, 128, 256):
+        die(f"session: --head-dim {args.head_dim} is not one of 64, 128 and "
+            "256")
     turn = args.prompt + args.infers_per_burst
     model = Sessions(args.batch, args.bursts * turn, args.layers, args.heads,
                      args.kv_heads, args.head_dim, args.page, args.cache,

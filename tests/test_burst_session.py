@@ -155,3 +155,30 @@ def test_session_refuses_sizes_below_one(name, capsys):
         infer_burst.main(["--model", "session", "--device", "cpu",
                           f"--{name}", "0"])
     assert f"--{name} 0" in capsys.readouterr().err
+
+
+@pytest.mark.parametrize("args,said", [
+    (("--infers-per-burst", "-3"), "--infers-per-burst -3"),
+    (("--heads", "0"), "--heads 0"),
+    (("--kv-heads", "0"), "--kv-heads 0"),
+    (("--heads", "6", "--kv-heads", "4"), "no multiple of --kv-heads 4"),
+    (("--head-dim", "80"), "--head-dim 80"),
+    (("--think-s", "-1"), "--think-s -1"),
+])
+def test_session_refuses_what_it_cannot_run(args, said, capsys):
+    """A turn of a prompt less some tokens had pages for those only."""
+    with pytest.raises(SystemExit):
+        infer_burst.main(["--model", "session", "--device", "cpu",
+                          "--prompt", "4", "--bursts", "2", "--layers", "1",
+                          "--batch", "1", *args])
+    assert said in capsys.readouterr().err
+
+
+def test_session_without_single_tokens(capsys):
+    infer_burst.main(["--model", "session", "--device", "cpu", "--batch",
+                      "1", "--bursts", "2", "--infers-per-burst", "0",
+                      "--prompt", "5", "--layers", "1", "--heads", "2",
+                      "--kv-heads", "2", "--head-dim", "64", "--think-s",
+                      "0"])
+    assert json.loads(capsys.readouterr().out.splitlines()[-1])[
+        "tokens"] == 10
