@@ -87,8 +87,8 @@ narrow_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 	const int kh = blockIdx.x % c.kv_heads;
 	const int block = blockIdx.x / c.kv_heads;
 
-	if (p.cover == 1)
-		cover_padding<T>(c, a, blockIdx.x, gridDim.x);
+	/* With starts there is always a narrow launch. */
+	cover_padding<T>(c, a, blockIdx.x, gridDim.x);
 
 	char *const k_lds = lds + wave * 2 * TILE * RB;
 	char *const v_lds = k_lds + TILE * RB;

@@ -75,8 +75,6 @@ wide_kernel(nvs_kv c, nvs_kv_attend_args a, nvs_plan p)
 	int64_t block;
 	int b;
 
-	if (p.cover == 2)
-		cover_padding<T>(c, a, blockIdx.x, gridDim.x);
 	if (c.starts) {
 		auto from = [&](int i) {
 			return (int64_t)c.starts[i] * group / WIDE_ROWS + i;

@@ -41,7 +41,6 @@ constexpr int nvs_narrow_waves(int dim, int size)
 	return dim * size > 256 ? 2 : 4;
 }
 
-
 /* How the work of one call is divided. */
 struct nvs_plan {
 	int narrow_rows; /* sequences with more rows go to the wide kernel */
@@ -51,8 +50,6 @@ struct nvs_plan {
 	int narrow_whole;  /* each of them has one sequence, undivided */
 	int wide_blocks;   /* blocks of rows, for one cached head */
 	int wide_parts;	   /* wide blocks that may divide one's keys */
-	int cover; /* the launch that sees to rows of no sequence: 1 narrow,
-		      2 wide */
 	uint64_t page_magic; /* key / page_size = key * magic >> shift */
 	int page_shift;
 	int near_slots; /* a tile's rows lie within 31 bits of each other */

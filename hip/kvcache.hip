@@ -348,9 +348,6 @@ nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, void *work,
 		if (p.wide_parts < 1)
 			p.wide_parts = 1;
 	}
-	if (c.starts)
-		p.cover = p.narrow_rows ? 1 : 2;
-
 	/* The parts' results, narrow before wide. */
 	const int64_t narrow = p.narrow_blocks > 1 && !p.narrow_whole ?
 				       (int64_t)p.narrow_blocks * 2 *

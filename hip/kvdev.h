@@ -23,7 +23,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
 typedef fp16_t fp16x2 __attribute__((ext_vector_type(2)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
@@ -34,7 +33,7 @@ template <> struct types<bf16_t> {
 	typedef bf16x2 x2;
 	typedef bf16x8 x8;
 	/* How far the running maximum of a softmax may lag behind, and what
-	 * is added to each exponent, in powers of two (softmax_* below). */
+	 * is added to each exponent, in powers of two (struct softmax). */
 	static constexpr float lag = 8.f, lift = 0.f;
 	static constexpr unsigned exponent = 0x7f807f80u, one = 0x00800080u;
 };
