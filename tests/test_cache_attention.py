@@ -279,6 +279,16 @@ def test_long_context_is_split(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("new,length,dim", [(20, 17403, 128),
+                                            (20, 17403, 256),
+                                            (33, 16500, 64)])
+def test_chunk_in_many_parts(gpu, new, length, dim):
+    """Sixteen parts and more, joined by four waves a row."""
+    check_attend(Step(gpu, [(new, length)], heads=4, kv_heads=1, dim=dim,
+                      page=64, uniform=True))
+
+
+@pytest.mark.gpu
 def test_unlike_lengths_in_one_batch(gpu):
     check_attend(Step(gpu, [(1, 4000), (1, 1), (1, 130), (0, 0), (1, 2900)],
                       heads=8, kv_heads=2, dim=128))
@@ -534,6 +544,45 @@ def test_weights_of_few_rows_keep_their_bits(device, dtype, cache, dim, new):
     cache, a = s.to()
     got = attend(cache, a["q"], a["table"], a["lens"])
     near(got, want.transpose(0, 1), 1.01 * tol.transpose(0, 1), "out")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cache", [None, E4M3])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 3, 16, 70])
+def test_what_is_no_number_in_each_type(device, dtype, cache, dim, new):
+    """Keys and values that are infinite or NaN spoil the rows that see
+    them, in the dimensions that they are in, and no others; e4m3 has NaN
+    only."""
+    s = Step(device, [(new, 90 + new)], dtype=dtype, cache=cache, dim=dim,
+             uniform=True, seed=dim + new)
+    cache0, a = s.to()
+
+    def run(k_at=(), v_at=()):
+        c = PagedCache(*(None if x is None else x.clone() for x in cache0))
+        for x, places in ((c.k, k_at), (c.v, v_at)):
+            for j, d, value in places:
+                bits = torch.tensor(value).to(x.dtype).view(
+                    torch.uint8 if cache else torch.int16)
+                x.view(bits.dtype)[s.slot(0, j)][:, d] = bits.to(device)
+        return attend(c, a["q"], a["table"], a["lens"])
+
+    clean = run()
+    last = 90 + new - 1  # seen by the last row only
+    values = (math.nan,) if cache else (math.nan, math.inf, -math.inf)
+    for value in values:
+        out = run(k_at=[(last, d, value) for d in range(dim)],
+                  v_at=[(last, d, value) for d in range(dim)])
+        assert torch.equal(out[:-1], clean[:-1])
+        assert not out[-1].isfinite().any()
+    spoilt = {3: values[0], 17: values[-1], dim - 1: values[len(values) // 2]}
+    out = run(v_at=[(j, d, x) for j in (30, last) for d, x in spoilt.items()])
+    for d, x in spoilt.items():
+        assert torch.equal(out[..., d].nan_to_num(),
+                           torch.full_like(out[..., d], x).nan_to_num())
+        assert out[..., d].isnan().all() or not math.isnan(x)
+        out[..., d] = clean[..., d]
+    assert torch.equal(out, clean)
 
 
 @pytest.mark.parametrize("new", [1, 6])
