@@ -7,6 +7,7 @@
  * the Python module's documentation is in this file, for tensors on the
  * CPU too; only what it names is launched, on the stream that it is given.
  */
+#include <ATen/MemoryOverlap.h>
 #include <torch/extension.h>
 
 #include <dlfcn.h>
@@ -127,6 +128,18 @@ void check_distinct(const char *name, const Tensor &t)
 			refuse(name, ": an expanded tensor cannot be written "
 				     "to (strides ",
 			       t.strides(), ")");
+}
+
+/* Nor is it in a place of `other`, as far as torch can tell cheaply: blocks
+ * read and write in any order. */
+void check_apart(const char *name, const Tensor &t, const Tensor &other,
+		 bool same_allowed = false)
+{
+	const at::MemOverlapStatus status = at::get_overlap_status(t, other);
+
+	if (status == at::MemOverlapStatus::Partial ||
+	    (status == at::MemOverlapStatus::Full && !same_allowed))
+		refuse(name, ": shares memory with other arguments");
 }
 
 void check_index(const char *name, const Tensor &t, int64_t n,
@@ -332,12 +345,20 @@ Maybe append(const Tensor &ck, const Tensor &cv, const Maybe &k_scale,
 		     { &k_scale, &v_scale, &q, &rotation, &q_out });
 	check_distinct("cache", ck);
 	check_distinct("cache", cv);
+	check_apart("cache", ck, cv);
+	for (const Tensor *t : { &k, &v }) {
+		check_apart("cache", ck, *t);
+		check_apart("cache", cv, *t);
+	}
 	a.fill = !q_out;
 	if (q && !q_out)
 		q_out = at::empty(q->sizes(), q->options());
 	else if (q) {
 		check_like("q_out", *q_out, *q, false);
 		check_distinct("q_out", *q_out);
+		check_apart("q_out", *q_out, *q, true);
+		for (const Tensor *t : { &k, &v, &ck, &cv })
+			check_apart("q_out", *q_out, *t);
 	}
 	if (c.total == 0 || !k.is_cuda())
 		return q_out;
@@ -398,6 +419,9 @@ std::pair<Tensor, Maybe> attend(const Tensor &ck, const Tensor &cv,
 	else {
 		check_like("out", *out, q, false);
 		check_distinct("out", *out);
+		check_apart("out", *out, q, true);
+		check_apart("out", *out, ck);
+		check_apart("out", *out, cv);
 	}
 	Maybe lse;
 

@@ -28,15 +28,17 @@ table[b, j // page_size].  An entry that is no page of the cache (-1, say)
 is allowed: what would be stored there is dropped, and what would be read
 there is not attended to.  The same holds for positions below zero, where
 lens is less than the rows, and behind the table.  Sequences may share
-pages that they only read; where two rows of a step have the same slot, what
-it then holds is of either.
+pages that they only read; where two rows of a step have the same slot, each
+value that it then holds is of either.
 
 Types.  bfloat16 or float16 rows; the cache in the rows' type, or in
 float8_e4m3fn with a float32 scale for each cached head (a value is stored
 as value / scale, and values over 448 as 448).  Head dimensions: multiples
 of 16 for `append`, 64, 128 or 256 for `attend`; a cached head serves
 heads / kv_heads query heads.  Tensors may be strided as long as each
-head's values are contiguous and begin at 16 bytes.
+head's values are contiguous and begin at 16 bytes.  What a call writes to
+(the cache, q_out, out) shares no memory with its other arguments, but that
+q_out and out may be q itself.
 
 Launches go to the current stream of the tensors' device, and their
 workspace comes from torch's allocator, so both may be captured.  Forward

@@ -1148,6 +1148,29 @@ def test_rows_of_no_shape_are_refused(device):
     refused("31 bits", lambda: attend(cache, heads, table, lens))
 
 
+def test_shared_memory_is_refused(device):
+    """Rows that are written where others are still read."""
+    s = Step(device, [(6, 30)], uniform=True)
+    cache, a = s.to()
+    k, v, table, lens = (a[n] for n in ("k", "v", "table", "lens"))
+    rows = torch.randn(7, 4, 64, device=device).to(s.q.dtype)
+    late, early = rows[1:], rows[:-1]
+    refused("out", lambda: attend(cache, late, table, lens, out=early))
+    refused("q_out", lambda: append(cache, k, v, table, lens, q=late,
+                                    q_out=early))
+    refused("cache", lambda: append(PagedCache(cache.k, cache.k), k, v,
+                                    table, lens))
+    held = cache.k.view(-1, 4, 64)[:6]
+    refused("out", lambda: attend(cache, a["q"], table, lens, out=held))
+    refused("q_out", lambda: append(cache, k, v, table, lens, q=a["q"],
+                                    q_out=held))
+    refused("cache", lambda: append(cache, cache.k.view(-1, 2, 64)[:6], v,
+                                    table, lens))
+    refused("q_out", lambda: append(cache, k, v, table, lens, q=k, q_out=v))
+    # Keys that are values too may be read.
+    attend(PagedCache(cache.k, cache.k), a["q"], table, lens)
+
+
 def test_scales_and_rotation_that_learn_are_refused(device):
     s = Step(device, [(2, 30)], uniform=True, cache=E4M3)
     cache, a = s.to()
