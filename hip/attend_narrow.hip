@@ -24,11 +24,12 @@ namespace {
  * once a tile (its page, its mask, the maximum over the lanes) would take
  * longer than its loads.
  *
- * One token over 120001 keys (8 cached heads of 128, bfloat16, 492 MB): 89
- * us, 5.5 TB/s; 64 tokens over up to 16384 keys each (2.36 GB): 423 us, 5.6
- * TB/s; the same loads without any arithmetic take as long, and plain loads
- * of the same pages reach 6.0 to 6.2 TB/s.  e4m3 (1.10 GB, rows of 128
- * bytes): 231 us, 4.8 TB/s.
+ * One token over 120001 keys (8 cached heads of 128, bfloat16, 492 MB): 91
+ * us, 5.4 TB/s; 64 tokens over up to 16384 keys each (2.36 GB): 431 us, 5.5
+ * TB/s (423 without any arithmetic; plain loads of the same pages reach 6.0
+ * to 6.2 TB/s).  e4m3 (1.10 GB, rows of 128 bytes): 230 us, 4.8 TB/s.  17
+ * to 32 rows with heads of 256 spill 48 registers (27 with e4m3): 8 x 8
+ * tokens over 5000 keys 128 us where 8 x 4 take 71.
  */
 template <typename T, typename C, int D, int NC, int W> struct narrow {
 	static constexpr int RB = D * sizeof(C); /* bytes of a row in LDS */

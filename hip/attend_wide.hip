@@ -8,7 +8,7 @@ namespace {
 
 /*
  * Bound by the matrix and vector instructions: a wave's tile is 32 products
- * of 32x32x16 (1024 cycles) and 186 vector instructions, 32 of them
+ * of 32x32x16 (1024 cycles) and 188 vector instructions, 32 of them
  * exponentials (870 cycles), which two waves of a SIMD overlap little: the
  * matrix units are busy 47 % of the time.
  *
@@ -19,8 +19,12 @@ namespace {
  * registers and lies in LDS as T, so that each value is widened once and
  * not by each wave.
  *
- * A chunk of 2048 tokens over 32049 keys (32 heads of 128, bfloat16): 1077
- * us, 970 TFLOP/s; prompts of 2048 from their first token: 175 us, 790.
+ * A chunk of 2048 tokens over 32049 keys (32 heads of 128, bfloat16): 1050
+ * us, 990 TFLOP/s (1040 to 1114 on one card or another); four prompts of
+ * 2048 from their first token: 171 us, 800.  Heads of 256: two chunks of
+ * 1500 in a window of 1024, 75 us, 336; 256 + 212 registers leave one wave
+ * a SIMD, and some 370 of a tile's 650 vector instructions move accumulators
+ * between the two files.
  * Slower, for the chunk: tiles of 32 keys 1254 us, with three blocks a CU
  * 1647; blocks of 256 rows 1495; scores of the next tile made between the
  * exponentials of this one 1290 and more, as the registers run out.

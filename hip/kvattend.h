@@ -8,9 +8,11 @@
  *
  *   narrow  up to 32 rows, as single tokens and drafts have: its waves
  *           share the rows and divide the keys, so that the cache streams
- *           through all of them; bound by the cache's bytes
+ *           through all of them; bound by the cache's bytes.  Weights meet
+ *           the values in two parts of the rows' type
  *   wide    128 rows, as chunks have: its waves divide the rows and share
- *           the keys in LDS; bound by the matrix products
+ *           the keys in LDS; bound by the matrix products.  Weights are
+ *           rounded once to the rows' type
  *
  * Both walk the keys in tiles with the running maximum and sum of the
  * softmax in 32 bits, and where there are few blocks of rows the keys are
@@ -34,7 +36,22 @@ constexpr int nvs_narrow_tile(int dim, int size)
 	return dim * size < 256 ? 64 : 32;
 }
 
-/* The fewest tiles that are worth a block of their own. */
+/*
+ * The fewest tiles that are worth a block of their own.
+ *
+ * Narrow: one for each of its waves.  With 2, one token over 611 keys takes
+ * 11.9 us instead of 11.6 and 8 of 900 keys 15.3 instead of 19.8, with 8
+ * 15.7 and 19.8; drafts of 6 over 5009 keys 21.2, 21.2 and 27.5.
+ *
+ * Wide: a join costs 4 to 5 us and the parts' traffic, and a block of heads
+ * of 256 fills a CU, so that twice as many blocks take two rounds: two
+ * chunks of 1500 in a window of 1024, 75 us with 16 or 32 and 106 with 4 or
+ * 8.  With heads of 128 fewer are better where there are few blocks: one
+ * sequence's 64 rows over 4000 keys 28, 25, 40 and 96 us with 4, 8, 16 and
+ * 32; 800 rows over 2000 keys 29, 28, 39 and 55; 2048 over 4000 59, 59, 64
+ * and 107; 8 sequences of 40 rows over 4000 36, 36, 42 and 95; long chunks
+ * do not care.
+ */
 constexpr int NARROW_LEAST = 4, WIDE_LEAST = 16;
 constexpr int nvs_narrow_waves(int dim, int size)
 {

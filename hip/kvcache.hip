@@ -87,7 +87,7 @@ __device__ __forceinline__ void store8(e4m3_t *p, const float *x)
  * every access is 16 bytes and a thread needs 8 cosines and sines only;
  * these are shared by a row's heads and come from cache.  15512 rows (32
  * query heads, 8 cached ones of 128, 389 MB): 85 us, 4.56 TB/s, as fast as
- * a copy of 4 GiB; one row: 3.4 us, a call 5.5.
+ * a copy of 4 GiB; one row: 3.0 us, a call 5.7.
  */
 template <typename T, typename C>
 __global__ __launch_bounds__(256) void append_kernel(nvs_kv c,
@@ -294,6 +294,18 @@ nvs_plan plan_of(const nvs_kv &c, const nvs_kv_attend_args &a, void *work,
 	const int64_t slot = c.k_slot > c.v_slot ? c.k_slot : c.v_slot;
 
 	p.near_slots = slot < (1ll << 30) / WIDE_TILE;
+	/* Two columns of 16 rows are what a narrow block holds.  For 32 rows
+	 * of each sequence, narrow and wide take: 8 sequences over 5000 keys,
+	 * heads of 128, 45 and 46 us, e4m3 33 and 46; one over 5000, 22 and
+	 * 35; 16 over 16000, 199 and 190; 8 over 5000 with heads of 256, 129
+	 * and 98 (registers spill in the narrow kernel), e4m3 88 and 95.  20
+	 * rows: 44 and 45.
+	 *
+	 * Among longer sequences one column only, as single tokens have.
+	 * Two: prompts and single tokens 398 us instead of 395; but 24
+	 * sequences of 4 to 32 rows over up to 5000 keys, in a step that may
+	 * have longer ones, 79 instead of 109, over up to 30000 246 instead of
+	 * 462. */
 	p.span = most_rows > 32 || most_rows <= 16 ? 16 : 32;
 	p.narrow_rows = most_rows <= 32 ? 0x7fffffff : c.starts ? 16 : 0;
 	p.joined_rows = (int)(most_rows < p.span ? most_rows : p.span);

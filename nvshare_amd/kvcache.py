@@ -140,6 +140,11 @@ def attend(cache: PagedCache, q: torch.Tensor, table: torch.Tensor,
     rows than that; the work is divided by it, and where it does not hold
     only the time suffers.
 
+    Scores, weights and sums are made in 32 bits.  A sequence of many rows
+    (more than 32 for a cached head, 16 beside longer ones) has its weights
+    rounded to the rows' type before they meet the values, one of few rows
+    keeps twice the bits.
+
     Returns [total, heads, dim], or goes into `out`, which may be q itself;
     with `return_lse` also the logarithm of each row's sum of exponentials,
     float32 [total, heads].  A row that sees no key gives zeros, and -inf.
