@@ -14,14 +14,14 @@ such a cache, as gfx950 kernels (hip/kvcache.hip):
 
 Sequences.  `table` [batch, per_seq] (int32) names each sequence's pages in
 order, `lens` [batch] (int32) the tokens that it has, those of this step
-included.  The step's rows q, k, v [total, heads, dim] hold the sequences
-one after the other: sequence b has rows starts[b] .. starts[b + 1] - 1
+included.  The step's rows q, k, v [total, heads, dim] hold the sequences one
+after the other: sequence b has rows starts[b] .. starts[b + 1] - 1
 (`starts` [batch + 1], int32, rising from its first entry; none and many
 rows alike; a sequence whose rows would pass total has none, and the rows
-are of no sequence), or, without `starts`, total / batch rows each.  Row i
-of its n rows has position lens[b] - n + i.  All three are read on the device when
-the kernels run, so a captured graph follows what they then hold; nothing
-may change them meanwhile.
+are of no sequence), or, without `starts`, total / batch rows each.  Row i of
+its n rows has position lens[b] - n + i.  All three are read on the device
+when the kernels run, so a captured graph follows what they then hold;
+nothing may change them meanwhile.
 
 Pages.  Position j of a sequence is in slot j % page_size of page
 table[b, j // page_size].  An entry that is no page of the cache (-1, say)
